@@ -116,6 +116,56 @@ int pal_fill_kv_pages_slots(const void* new_keys, const void* new_values, void* 
                             int num_kv_heads, int head_dim, int tokens_per_page,
                             int64_t num_pages, int dtype, void* stream);
 
+/* ---- rotary positions --------------------------------------------------------------------- */
+/* No counterpart in the reference, whose callers rotate queries and keys before they call it.
+ *
+ * Frequency i < num_freqs turns one pair of elements (a, b) of every head of token t by the angle
+ * positions[axis(i)][t] * inv_freq[i]: a' = magnitude * (a cos - b sin), b' = magnitude * (b cos + a sin).
+ * Elements from 2 * num_freqs on pass through unchanged.  The angle is formed and reduced in 64 bits, so that far
+ * positions keep the accuracy of near ones; the rotation is fp32, rounded once. */
+#define PAL_PAIRING_HALF 0        /* the pair of frequency i is elements (i, i + num_freqs) */
+#define PAL_PAIRING_ADJACENT 1    /* ... elements (2i, 2i + 1) */
+#define PAL_SECTIONS_BLOCKED 0    /* axis 0 has the first sections[0] frequencies, axis 1 the next sections[1], ... */
+#define PAL_SECTIONS_INTERLEAVED 1 /* frequency i is axis i % num_axes, until an axis other than 0 has its sections[];
+                                     axis 0 has all others */
+#define PAL_MAX_ROTARY_AXES 4
+typedef struct pal_rotation {
+  const void* positions;          /* device, [num_axes][num_tokens] (any axis stride), int32 or int64; may be negative */
+  int64_t positions_axis_stride;  /* in elements */
+  const float* inv_freq;          /* device, [num_freqs] */
+  float magnitude;                /* factor on sine and cosine (1 for the plain rotation) */
+  int32_t num_freqs;
+  int32_t num_axes;               /* 1 to PAL_MAX_ROTARY_AXES */
+  int32_t sections[PAL_MAX_ROTARY_AXES]; /* frequencies of each axis, their sum num_freqs; unused with one axis */
+  int32_t section_order;
+  int32_t pairing;
+  int32_t positions_64bit;
+} pal_rotation;
+
+/* [token][head][element] rows with unit element stride; strides count elements and may be those of a slice of a wider
+ * matrix. */
+typedef struct pal_rows {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+} pal_rows;
+
+/* out[t, h, :] = rotation of x[t, h, :].  out may be x (same strides); otherwise the two must not overlap. */
+int pal_rotary_embedding(const pal_rows* x, const pal_rows* out, const pal_rotation* rotation, int64_t num_tokens,
+                         int num_heads, int head_dim, int dtype, void* stream);
+
+/* Append with rotation: the keys are rotated on their way into the K pool, the values go into the V pool as they are, and
+ * (when num_q_heads > 0) the queries are rotated into queries_out, which may be queries - one launch.  Tokens are addressed
+ * by slot_mapping (int64), or, when that is null, by page_table / write_positions / query_to_seq_map, with the rules of
+ * pal_fill_kv_pages[_slots]: a token whose destination is out of range is skipped (its query is still rotated).
+ * Destinations must differ from one another.  head_dim is a multiple of 8, at most 256. */
+int pal_fill_kv_pages_rotary(const pal_rows* new_keys, const pal_rows* new_values, const pal_rows* queries,
+                             const pal_rows* queries_out, void* k_pool, void* v_pool, const int64_t* slot_mapping,
+                             const void* page_table, const int32_t* write_positions, const void* query_to_seq_map,
+                             const pal_rotation* rotation, int64_t num_tokens, int num_seqs, int num_q_heads,
+                             int num_kv_heads, int head_dim, int tokens_per_page, int64_t num_pages,
+                             int max_pages_per_seq, int dtype, void* stream);
+
 /* ---- paged_attention_decode --------------------------------------------------------------- */
 /* Bytes of device workspace pal_paged_attention_decode needs for this problem; depends on
  * partition_pages (see below).  Always >= 256. */

@@ -7,6 +7,7 @@ blocks used for multi-GPU long-context decode.
 from . import pal_core, sharding  # noqa: F401
 from .ops import (  # noqa: F401
     fill_kv_pages,
+    fill_kv_pages_rotary,
     get_k_cache_shape,
     get_k_cache_stripe_size,
     get_optimal_page_size,
@@ -20,10 +21,12 @@ from .ops import (  # noqa: F401
     paged_attention_decode_partials,
     paged_attention_prefill,
     paged_attention_prefill_ragged,
+    rotary_embedding,
 )
 
 __all__ = [
     "fill_kv_pages",
+    "fill_kv_pages_rotary",
     "get_k_cache_shape",
     "get_k_cache_stripe_size",
     "get_optimal_page_size",
@@ -37,4 +40,5 @@ __all__ = [
     "paged_attention_decode_partials",
     "paged_attention_prefill",
     "paged_attention_prefill_ragged",
+    "rotary_embedding",
 ]

@@ -24,10 +24,29 @@ PAL_DTYPE_BF16 = 1
 PAL_OUT_F32 = 0x100
 PAL_STATIC_SCRATCH_BYTES = 16 * 1024 * 1024
 
+PAL_MAX_ROTARY_AXES = 4
+
 PAL_DECODE_SINGLE_PASS = 0
 PAL_DECODE_AUTO = -1
 
 _P = c_void_p
+
+
+class Rows(ctypes.Structure):
+    """``pal_rows``: [token][head][element] rows, strides in elements."""
+
+    _fields_ = [("data", c_void_p), ("token_stride", c_int64), ("head_stride", c_int64)]
+
+
+class Rotation(ctypes.Structure):
+    """``pal_rotation``: positions, frequencies and the arrangement of axes and pairs."""
+
+    _fields_ = [("positions", c_void_p), ("positions_axis_stride", c_int64), ("inv_freq", c_void_p), ("magnitude", c_float),
+                ("num_freqs", ctypes.c_int32), ("num_axes", ctypes.c_int32), ("sections", ctypes.c_int32 * PAL_MAX_ROTARY_AXES),
+                ("section_order", ctypes.c_int32), ("pairing", ctypes.c_int32), ("positions_64bit", ctypes.c_int32)]
+
+
+_ROWS, _ROTATION = ctypes.POINTER(Rows), ctypes.POINTER(Rotation)
 # name -> (restype, argtypes); mirrors include/pal_b200.h one to one
 SIGNATURES = {
     "pal_last_error": (c_char_p, []),
@@ -38,6 +57,11 @@ SIGNATURES = {
     "pal_get_v_cache_shape": (c_int, [c_int64, c_int, c_int, c_int, c_int, ctypes.POINTER(c_int64)]),
     "pal_fill_kv_pages": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int64, c_int, c_int, _P]),
     "pal_fill_kv_pages_slots": (c_int, [_P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int64, c_int, _P]),
+    "pal_rotary_embedding": (c_int, [_ROWS, _ROWS, _ROTATION, c_int64, c_int, c_int, c_int, _P]),
+    "pal_fill_kv_pages_rotary": (
+        c_int,
+        [_ROWS, _ROWS, _ROWS, _ROWS, _P, _P, _P, _P, _P, _P, _ROTATION, c_int64, c_int, c_int, c_int, c_int, c_int, c_int64, c_int, c_int, _P],
+    ),
     "pal_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "pal_decode_auto_partition_pages": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "pal_paged_attention_decode": (

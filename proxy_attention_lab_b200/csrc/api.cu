@@ -198,6 +198,146 @@ int pal_fill_kv_pages_slots(const void* new_keys, const void* new_values, void* 
   return fill_common(a, dtype, stream);
 }
 
+static bool rotation_args(const char* what, const pal_rotation* r, int64_t num_tokens, int head_dim, RotationArgs* out) {
+  if (!r || !r->inv_freq || (num_tokens > 0 && !r->positions)) {
+    set_error("%s: the rotation needs positions and inv_freq", what);
+    return false;
+  }
+  if (r->num_freqs <= 0 || r->num_freqs > head_dim / 2) {
+    set_error("%s: %d frequencies rotate %lld elements, a head has %d", what, r->num_freqs, 2LL * r->num_freqs, head_dim);
+    return false;
+  }
+  if (r->num_axes < 1 || r->num_axes > PAL_MAX_ROTARY_AXES) {
+    set_error("%s: num_axes must be 1 to %d, got %d", what, PAL_MAX_ROTARY_AXES, r->num_axes);
+    return false;
+  }
+  if ((r->pairing != PAL_PAIRING_HALF && r->pairing != PAL_PAIRING_ADJACENT) ||
+      (r->section_order != PAL_SECTIONS_BLOCKED && r->section_order != PAL_SECTIONS_INTERLEAVED)) {
+    set_error("%s: unknown pairing (%d) or section order (%d)", what, r->pairing, r->section_order);
+    return false;
+  }
+  if (r->num_axes > 1) {
+    long long sum = 0;
+    for (int a = 0; a < r->num_axes; ++a) {
+      const int n = r->sections[a];
+      sum += n;
+      // interleaved: the last frequency of axis a is a + num_axes * (n - 1)
+      const bool fits = r->section_order == PAL_SECTIONS_BLOCKED || a == 0 || n <= 0 || a + (long long)r->num_axes * (n - 1) < r->num_freqs;
+      if (n < 0 || !fits) {
+        set_error("%s: section %d (%d frequencies) does not fit %d frequencies over %d axes", what, a, n, r->num_freqs, r->num_axes);
+        return false;
+      }
+    }
+    if (sum != r->num_freqs) {
+      set_error("%s: the sections hold %lld frequencies, inv_freq %d", what, sum, r->num_freqs);
+      return false;
+    }
+  }
+  out->positions = r->positions;
+  out->positions_axis_stride = r->positions_axis_stride;
+  out->inv_freq = r->inv_freq;
+  out->num_freqs = r->num_freqs;
+  out->num_axes = r->num_axes;
+  for (int a = 0; a < kMaxRotaryAxes; ++a) out->sections[a] = r->sections[a];
+  out->section_order = r->section_order;
+  out->pairing = r->pairing;
+  out->positions_64bit = r->positions_64bit;
+  out->magnitude = r->magnitude;
+  return true;
+}
+
+static bool rows_arg(const char* what, const char* name, const pal_rows* r, RowsView* out) {
+  if (!r || !r->data) {
+    set_error("%s: %s is null", what, name);
+    return false;
+  }
+  if (reinterpret_cast<uintptr_t>(r->data) & 1) {
+    set_error("%s: %s must be 2-byte aligned", what, name);
+    return false;
+  }
+  *out = RowsView{r->data, (long long)r->token_stride, (long long)r->head_stride};
+  return true;
+}
+
+int pal_rotary_embedding(const pal_rows* x, const pal_rows* out, const pal_rotation* rotation, int64_t num_tokens, int num_heads,
+                         int head_dim, int dtype, void* stream) {
+  const char* what = "rotary_embedding";
+  if (!check_dtype(dtype, what)) return PAL_ERR_UNSUPPORTED;
+  if (num_tokens < 0 || num_heads < 0 || head_dim <= 0) {
+    set_error("%s: token and head counts must not be negative, head_dim must be positive", what);
+    return PAL_ERR_BAD_ARG;
+  }
+  RotaryArgs a{};
+  if (!rotation_args(what, rotation, num_tokens, head_dim, &a.rot)) return PAL_ERR_BAD_ARG;
+  if (num_tokens == 0 || num_heads == 0) return PAL_OK;
+  RowsView o;
+  if (!rows_arg(what, "x", x, &a.q) || !rows_arg(what, "out", out, &o)) return PAL_ERR_BAD_ARG;
+  a.q_out = RowsOut{out->data, o.token_stride, o.head_stride};
+  a.fill.num_tokens = num_tokens;
+  a.fill.head_dim = head_dim;
+  a.num_q_heads = num_heads;
+  a.dtype = dtype;
+  return cuda_rc(launch_rotary(a, (cudaStream_t)stream), what);
+}
+
+int pal_fill_kv_pages_rotary(const pal_rows* new_keys, const pal_rows* new_values, const pal_rows* queries,
+                             const pal_rows* queries_out, void* k_pool, void* v_pool, const int64_t* slot_mapping,
+                             const void* page_table, const int32_t* write_positions, const void* query_to_seq_map,
+                             const pal_rotation* rotation, int64_t num_tokens, int num_seqs, int num_q_heads, int num_kv_heads,
+                             int head_dim, int tokens_per_page, int64_t num_pages, int max_pages_per_seq, int dtype, void* stream) {
+  const char* what = "fill_kv_pages_rotary";
+  if (!check_dtype(dtype, what)) return PAL_ERR_UNSUPPORTED;
+  if (num_tokens < 0 || num_pages < 0 || num_q_heads < 0 || num_seqs < 0 || max_pages_per_seq < 0) {
+    set_error("%s: negative token, page, sequence or head count", what);
+    return PAL_ERR_BAD_ARG;
+  }
+  if (num_kv_heads <= 0 || head_dim <= 0 || tokens_per_page <= 0) {
+    set_error("%s: num_kv_heads, head_dim and tokens_per_page must be positive", what);
+    return PAL_ERR_BAD_ARG;
+  }
+  if (head_dim % 8 != 0 || head_dim > 256) {
+    set_error("%s: head_dim (%d) must be a multiple of 8, at most 256", what, head_dim);
+    return PAL_ERR_UNSUPPORTED;
+  }
+  RotaryArgs a{};
+  if (!rotation_args(what, rotation, num_tokens, head_dim, &a.rot)) return PAL_ERR_BAD_ARG;
+  if (num_tokens == 0) return PAL_OK;
+  if (!rows_arg(what, "new_keys", new_keys, &a.k) || !rows_arg(what, "new_values", new_values, &a.v)) return PAL_ERR_BAD_ARG;
+  if (num_q_heads > 0) {
+    RowsView o;
+    if (!rows_arg(what, "queries", queries, &a.q) || !rows_arg(what, "queries_out", queries_out, &o)) return PAL_ERR_BAD_ARG;
+    a.q_out = RowsOut{queries_out->data, o.token_stride, o.head_stride};
+  }
+  if (!slot_mapping && (!page_table || !write_positions || !query_to_seq_map) && max_pages_per_seq > 0) {
+    set_error("%s: slot_mapping, or page_table, write_positions and query_to_seq_map are required", what);
+    return PAL_ERR_BAD_ARG;
+  }
+  if (num_pages > 0 && (!k_pool || !v_pool)) {
+    set_error("%s: null pool pointer", what);
+    return PAL_ERR_BAD_ARG;
+  }
+  if (!aligned16(k_pool) || !aligned16(v_pool)) {
+    set_error("%s: the pools must be 16-byte aligned", what);
+    return PAL_ERR_BAD_ARG;
+  }
+  a.fill.k_pool = k_pool;
+  a.fill.v_pool = v_pool;
+  a.fill.slot_mapping = slot_mapping;
+  a.fill.page_table = page_table;
+  a.fill.write_positions = write_positions;
+  a.fill.query_to_seq_map = query_to_seq_map;
+  a.fill.num_tokens = num_tokens;
+  a.fill.num_seqs = num_seqs;
+  a.fill.num_kv_heads = num_kv_heads;
+  a.fill.head_dim = head_dim;
+  a.fill.tokens_per_page = tokens_per_page;
+  a.fill.num_pages = num_pages;
+  a.fill.max_pages_per_seq = max_pages_per_seq;
+  a.num_q_heads = num_q_heads;
+  a.dtype = dtype;
+  return cuda_rc(launch_rotary(a, (cudaStream_t)stream), what);
+}
+
 size_t pal_decode_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
                                   int tokens_per_page, int max_pages_per_seq, int partition_pages) {
   if (num_seqs < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0) return sizeof(WorkspaceHeader);

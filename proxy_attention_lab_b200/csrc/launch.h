@@ -58,6 +58,41 @@ struct FillArgs {
   int max_pages_per_seq;
 };
 
+// Rows [token][head][element] with unit element stride, strides counted in elements.
+struct RowsView {
+  const void* data = nullptr;
+  long long token_stride = 0, head_stride = 0;
+};
+struct RowsOut {
+  void* data = nullptr;
+  long long token_stride = 0, head_stride = 0;
+};
+
+constexpr int kMaxRotaryAxes = 4;
+struct RotationArgs {
+  const void* positions;  // [num_axes][tokens], int32 or int64
+  long long positions_axis_stride;
+  const float* inv_freq;  // [num_freqs]
+  int num_freqs;          // half of the rotated elements of a head
+  int num_axes;
+  int sections[kMaxRotaryAxes];  // frequencies of each axis (unused with one axis)
+  int section_order;             // 0 = blocked, 1 = interleaved
+  int pairing;                   // 0 = (i, i + num_freqs), 1 = (2i, 2i + 1)
+  int positions_64bit;
+  float magnitude;
+};
+
+// Rotated queries and / or an append of rotated keys and of values (k.data set: then v and the pools and addresses of `fill`
+// are too).  fill carries the token count, the head count and size and the addressing; its new_keys / new_values are unused.
+struct RotaryArgs {
+  RotationArgs rot;
+  RowsView q, k, v;
+  RowsOut q_out;
+  FillArgs fill;
+  int num_q_heads;
+  int dtype;
+};
+
 struct DecodeArgs {
   const void* queries;
   const void* k_pool;
@@ -117,6 +152,7 @@ struct PrefillArgs {
 // Each returns a cudaError_t value as int (0 = success) or a negative PAL_ERR_* code, and
 // leaves a message via set_error() on failure.
 int launch_fill(const FillArgs& a, cudaStream_t stream);
+int launch_rotary(const RotaryArgs& a, cudaStream_t stream);
 int launch_decode(const DecodeArgs& a, cudaStream_t stream);
 // Strided views of a set of partial triples (element strides): partition j of row r has its m / l at
 // m[j * part_stride_ml + r * row_stride_ml] and its acc row at acc + j * part_stride_acc + r * row_stride_acc.

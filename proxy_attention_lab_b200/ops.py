@@ -278,6 +278,220 @@ def fill_kv_pages(
 
 
 # ---------------------------------------------------------------------------------------------
+# rotary positions (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------------
+ROTARY_PAIRING = {"half": 0, "adjacent": 1}
+SECTION_ORDER = {"blocked": 0, "interleaved": 1}
+
+
+def _rows(name: str, t: torch.Tensor, shape, dtype, device) -> _lib.Rows:
+    """A [tokens, heads, head_dim] tensor as rows with strides; the elements of a head have to be neighbours."""
+    _need_cuda(name, t)
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {list(shape)} of {dtype} on {device}, got {list(t.shape)} of {t.dtype} on {t.device}")
+    if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+    return _lib.Rows(_ptr(t), t.stride(0), t.stride(1))
+
+
+def _check_distinct_rows(name: str, t: torch.Tensor) -> None:
+    """Refuse an output whose rows share memory (an expanded tensor)."""
+    (n0, n1, n2), (s0, s1, _) = t.shape, t.stride()
+    pairs = sorted([(s1, n1), (s0, n0)])
+    need = n2
+    for stride, n in pairs:
+        if n > 1:
+            if stride < need:
+                raise ValueError(f"the rows of {name} overlap")
+            need = stride * (n - 1) + need
+
+
+def _rotation(positions, inv_freq, tokens: int, head_dim: int, sections, section_order: str, pairing: str, magnitude: float, device):
+    """The checked ``pal_rotation`` of a call and the tensors it points to (which have to outlive the launch)."""
+    _need_cuda("positions", positions)
+    _need_cuda("inv_freq", inv_freq)
+    if positions.device != device or inv_freq.device != device:
+        raise ValueError(f"positions and inv_freq must be on {device}")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
+        raise ValueError("inv_freq must be a 1-D float32 tensor")
+    if pairing not in ROTARY_PAIRING:
+        raise ValueError(f"pairing must be one of {sorted(ROTARY_PAIRING)}, got {pairing!r}")
+    if section_order not in SECTION_ORDER:
+        raise ValueError(f"section_order must be one of {sorted(SECTION_ORDER)}, got {section_order!r}")
+    half = inv_freq.shape[0]
+    if not 0 < 2 * half <= head_dim:
+        raise ValueError(f"inv_freq must hold 1 to head_dim / 2 = {head_dim // 2} frequencies, got {half}")
+    sections = [half] if sections is None else [int(n) for n in sections]
+    axes = len(sections)
+    if not 1 <= axes <= _lib.PAL_MAX_ROTARY_AXES:
+        raise ValueError(f"there are 1 to {_lib.PAL_MAX_ROTARY_AXES} position axes, got {axes} sections")
+    if min(sections) < 0 or sum(sections) != half:
+        raise ValueError(f"the sections {sections} must add up to the {half} frequencies of inv_freq")
+    if section_order == "interleaved" and any(n > 0 and a + axes * (n - 1) >= half for a, n in enumerate(sections) if a):
+        raise ValueError(f"the sections {sections} cannot be interleaved: an axis runs past the {half} frequencies")
+    if tuple(positions.shape) != (axes, tokens) and not (axes == 1 and tuple(positions.shape) == (tokens,)):
+        raise ValueError(f"positions must be [{tokens}] or [{axes}, {tokens}] (one row per section), got {list(positions.shape)}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        if positions.dtype.is_floating_point or positions.dtype in (torch.bool, torch.complex64, torch.complex128):
+            raise TypeError(f"positions must be an integer tensor, got {positions.dtype}")
+        positions = positions.to(torch.int64)
+    if positions.numel() and positions.shape[-1] > 1 and positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    inv_freq = _contig(inv_freq)
+    rot = _lib.Rotation(_ptr(positions), positions.stride(0) if positions.dim() == 2 else 0, inv_freq.data_ptr(), float(magnitude), half, axes,
+                        (_lib.ctypes.c_int32 * _lib.PAL_MAX_ROTARY_AXES)(*sections), SECTION_ORDER[section_order], ROTARY_PAIRING[pairing],
+                        1 if positions.dtype == torch.int64 else 0)
+    return rot, (positions, inv_freq)
+
+
+def rotary_embedding(x, positions, inv_freq, *, sections=None, section_order: str = "blocked", pairing: str = "half",
+                     magnitude: float = 1.0, out=None, stream=None):
+    """Rotate the heads of ``x [T, H, D]`` by their tokens' positions.
+
+    Frequency ``i`` of ``inv_freq [R/2]`` (float32) turns one pair of elements of every head of token ``t`` by the angle
+    ``positions[t] * inv_freq[i]``: elements ``(i, i + R/2)`` with ``pairing="half"``, ``(2i, 2i + 1)`` with ``"adjacent"``.
+    Elements from ``R`` on pass through; ``magnitude`` scales the rotated ones.  ``positions`` is ``[T]`` (integers of any
+    sign), or ``[A, T]`` with ``sections``, the number of frequencies that each of the ``A <= 4`` axes (time, height, width,
+    ...) turns: the first ``sections[0]`` belong to axis 0 and so on (``section_order="blocked"``), or frequency ``i``
+    belongs to axis ``i % A`` until that axis has its number, and the rest to axis 0 (``"interleaved"``).  The angle is
+    taken in 64 bits, so far positions are as accurate as near ones.
+
+    ``x`` may be a strided view (a column range of a fused projection); the result is contiguous, or ``out`` (which may be
+    ``x``, but must not overlap it otherwise).  Negated positions undo the rotation; the gradient of ``x`` is the rotation of
+    the output's gradient by the negated positions.
+    """
+    _need_cuda("x", x)
+    if x.dim() != 3:
+        raise ValueError("x must be 3-D [tokens, heads, head_dim]")
+    code = _dtype_code(x.dtype)
+    T, H, D = x.shape
+    dev = x.device
+    with _Scope(dev, stream) as sp:
+        rot, keep = _rotation(positions, inv_freq, T, D, sections, section_order, pairing, magnitude, dev)
+        src = _rows("x", x, x.shape, x.dtype, dev)
+        if out is None:
+            out = torch.empty((T, H, D), dtype=x.dtype, device=dev)
+        dst = _rows("out", out, x.shape, x.dtype, dev)
+        _check_distinct_rows("out", out)
+        _lib.check(lib.pal_rotary_embedding(src, dst, rot, T, H, D, code, sp))
+    return out
+
+
+def fill_kv_pages_rotary(
+    new_keys,
+    new_values,
+    global_key_pool,
+    global_value_pool,
+    page_table=None,
+    current_token_write_positions=None,
+    query_to_seq_map=None,
+    *,
+    inv_freq,
+    positions=None,
+    queries=None,
+    slot_mapping=None,
+    sections=None,
+    section_order: str = "blocked",
+    pairing: str = "half",
+    magnitude: float = 1.0,
+    queries_out=None,
+    inplace: bool = True,
+    stream=None,
+):
+    """``fill_kv_pages`` of rotated keys and of values, and the rotation of the queries, in one launch.
+
+    ``new_keys / new_values [T, Hkv, D]`` and ``queries [T, Hq, D]`` may be strided views of a fused projection.  The keys
+    are rotated as by :func:`rotary_embedding` on their way into the pool.  Tokens are addressed as in :func:`fill_kv_pages`
+    (page table, write positions and sequence map, or ``slot_mapping``); a token whose destination is out of range is
+    skipped, its query is rotated all the same.  Destinations must differ from one another.  ``positions`` defaults to the
+    write positions (one axis).
+
+    Returns ``(k_pool, v_pool)``, or ``(k_pool, v_pool, rotated queries)`` when ``queries`` is given (written to
+    ``queries_out``, which may be ``queries``, if given).  The pools are updated in place unless ``inplace=False``.
+    """
+    if slot_mapping is None and page_table is not None and current_token_write_positions is None and query_to_seq_map is None:
+        slot_mapping, page_table = page_table, None
+    for name, t in (("new_keys", new_keys), ("new_values", new_values), ("global_key_pool", global_key_pool),
+                    ("global_value_pool", global_value_pool)):
+        _need_cuda(name, t)
+    if global_key_pool.dim() != 5:
+        raise ValueError("global_key_pool must be 5-D [pages, kv_heads, head_dim/x, tokens_per_page, x]")
+    if global_value_pool.dim() != 4:
+        raise ValueError("global_value_pool must be 4-D [pages, kv_heads, head_dim, tokens_per_page]")
+    code = _dtype_code(global_value_pool.dtype)
+    num_pages, hkv, d, tpp = global_value_pool.shape
+    if tuple(global_key_pool.shape) != (num_pages, hkv, d // 8, tpp, 8) or global_key_pool.dtype != global_value_pool.dtype:
+        raise ValueError("global_key_pool shape and dtype must match global_value_pool")
+    if not (global_key_pool.is_contiguous() and global_value_pool.is_contiguous()):
+        raise ValueError("the page pools must be contiguous")
+    if new_keys.dim() != 3:
+        raise ValueError(f"new_keys / new_values must be [T, {hkv}, {d}]")
+    T = new_keys.shape[0]
+    dev, dtype = global_value_pool.device, global_value_pool.dtype
+    if global_key_pool.device != dev:
+        raise ValueError("both pools must be on one device")
+    if slot_mapping is not None:
+        _need_cuda("slot_mapping", slot_mapping)
+        if slot_mapping.numel() != T:
+            raise ValueError("slot_mapping must have one entry per new token")
+        if positions is None:
+            raise ValueError("positions are required with slot_mapping")
+        addresses = (("slot_mapping", slot_mapping),)
+    else:
+        if page_table is None or current_token_write_positions is None or query_to_seq_map is None:
+            raise ValueError("page_table, current_token_write_positions and query_to_seq_map are required")
+        addresses = (("page_table", page_table), ("current_token_write_positions", current_token_write_positions),
+                     ("query_to_seq_map", query_to_seq_map))
+        for name, t in addresses:
+            _need_cuda(name, t)
+        if page_table.dim() != 2:
+            raise ValueError("page_table must be 2-D [num_sequences, max_logical_pages]")
+        if current_token_write_positions.numel() != T or query_to_seq_map.numel() != T:
+            raise ValueError("write positions and query_to_seq_map must have one entry per new token")
+    for name, t in addresses:
+        if t.device != dev:
+            raise ValueError(f"{name} must be on {dev}")
+    if queries is None and queries_out is not None:
+        raise ValueError("queries_out without queries")
+    with _Scope(dev, stream) as sp:
+        if slot_mapping is None:
+            pt = _index32("page_table", page_table)
+            wp = _index32("current_token_write_positions", current_token_write_positions)
+            sm = _index32("query_to_seq_map", query_to_seq_map)
+            where = (None, _ptr(pt), wp.data_ptr(), sm.data_ptr())
+            num_seqs, max_pages = pt.shape
+            if positions is None:
+                positions = wp.reshape(T).view(torch.int32)
+        else:
+            if slot_mapping.dtype.is_floating_point:
+                raise TypeError(f"slot_mapping must be an integer tensor, got {slot_mapping.dtype}")
+            slots = _contig(slot_mapping.to(torch.int64))
+            where = (slots.data_ptr(), None, None, None)
+            num_seqs = max_pages = 0
+        rot, keep = _rotation(positions, inv_freq, T, d, sections, section_order, pairing, magnitude, dev)
+        k = _rows("new_keys", new_keys, (T, hkv, d), dtype, dev)
+        v = _rows("new_values", new_values, (T, hkv, d), dtype, dev)
+        q = qo = None
+        hq = 0
+        if queries is not None:
+            _need_cuda("queries", queries)
+            if queries.dim() != 3:
+                raise ValueError("queries must be 3-D [tokens, heads, head_dim]")
+            hq = queries.shape[1]
+            q = _rows("queries", queries, (T, hq, d), dtype, dev)
+            if queries_out is None:
+                queries_out = torch.empty((T, hq, d), dtype=dtype, device=dev)
+            qo = _rows("queries_out", queries_out, (T, hq, d), dtype, dev)
+            _check_distinct_rows("queries_out", queries_out)
+        if not inplace:
+            global_key_pool = global_key_pool.clone()
+            global_value_pool = global_value_pool.clone()
+        _lib.check(lib.pal_fill_kv_pages_rotary(k, v, q, qo, _ptr(global_key_pool), _ptr(global_value_pool), *where, rot, T, num_seqs, hq, hkv,
+                                                d, tpp, num_pages, max_pages, code, sp))
+    return (global_key_pool, global_value_pool) if queries is None else (global_key_pool, global_value_pool, queries_out)
+
+
+# ---------------------------------------------------------------------------------------------
 # paged_attention_decode (src/proxy_attention_lab/ops.py:42-84, src/pal_core/src/ops.cpp:36-108)
 # ---------------------------------------------------------------------------------------------
 def _decode_shapes(queries, k_cache_pool, v_cache_pool, page_table, sequence_lengths):
