@@ -345,6 +345,31 @@ int pal_paged_attention_prefill_ragged(const void* q_prompt, const void* k_promp
                                        int max_pages_per_seq, float scale, int dtype, int impl, void* workspace,
                                        size_t workspace_bytes, void* stream);
 
+/* ---- attention of new tokens over the paged cache alone ----------------------------------- */
+/* No counterpart in the reference, whose prefill takes the new tokens' keys and values as dense tensors beside the paged
+ * history (src/pal_core/src/paged_attention_prefill_primitive.cpp:63-167).  Here they have been appended to the pages before
+ * the call, and sequence_lengths counts them.
+ *
+ * queries: [total_tokens][Hq][D] rows (token and head strides in elements, multiples of 8; 16-byte aligned); sequence s owns
+ * rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (device array of num_seqs + 1 int32 offsets, not decreasing), or, when
+ * cu_seqlens is null, total_tokens / num_seqs rows each.  Row i of n stands at position L - n + i, L = sequence_lengths[s].
+ * It sees the keys up to its own position, and with window > 0 only the last `window` of them; with causal = 0 (window must
+ * be 0) all L keys.  A row that sees no key becomes zeros.  out [total_tokens, Hq, D] in the query dtype, or float32 with
+ * dtype | PAL_OUT_F32; rows that belong to no sequence are left as they were.  Page ids are clamped to [0, num_pages); pages
+ * that hold no visible key are not read.  scale <= 0 selects 1/sqrt(D).
+ *
+ * scratch: pal_chunk_scratch_bytes() bytes of device memory, 256-byte aligned, with any contents, for one call at a time.
+ * status: one 32-bit word of device memory that is zero before the first use and takes the error code of a wait that gave
+ * up (pal_check_status reads and clears it when it is the second word of a workspace); may be null, and shared by calls
+ * that overlap. */
+size_t pal_chunk_scratch_bytes(int64_t total_tokens, int num_q_heads, int num_kv_heads, int head_dim);
+int pal_paged_attention_chunk(const void* queries, int64_t query_token_stride, int64_t query_head_stride,
+                              const void* k_pool, const void* v_pool, const void* page_table,
+                              const int32_t* sequence_lengths, const int32_t* cu_seqlens, void* out, int num_seqs,
+                              int64_t total_tokens, int num_q_heads, int num_kv_heads, int head_dim, int tokens_per_page,
+                              int64_t num_pages, int max_pages_per_seq, float scale, int causal, int window, int dtype,
+                              void* scratch, size_t scratch_bytes, void* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

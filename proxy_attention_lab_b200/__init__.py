@@ -16,6 +16,7 @@ from .ops import (  # noqa: F401
     lse_combine,
     lse_combine_packed,
     paged_attention,
+    paged_attention_chunk,
     paged_attention_decode,
     paged_attention_decode_append,
     paged_attention_decode_partials,
@@ -35,6 +36,7 @@ __all__ = [
     "lse_combine",
     "lse_combine_packed",
     "paged_attention",
+    "paged_attention_chunk",
     "paged_attention_decode",
     "paged_attention_decode_append",
     "paged_attention_decode_partials",

@@ -100,6 +100,12 @@ SIGNATURES = {
         [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int64, c_int, c_float, c_int, c_int, _P, c_size_t,
          ctypes.POINTER(c_void_p), c_int, c_int, c_int64, _P],
     ),
+    "pal_chunk_scratch_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
+    "pal_paged_attention_chunk": (
+        c_int,
+        [_P, c_int64, c_int64, _P, _P, _P, _P, _P, _P, c_int, c_int64, c_int, c_int, c_int, c_int, c_int64, c_int, c_float, c_int, c_int,
+         c_int, _P, c_size_t, _P, _P],
+    ),
     "pal_lse_combine_packed": (c_int, [_P, _P, c_int, c_int64, c_int, c_int, _P]),
     "pal_workspace_init": (c_int, [_P, c_size_t, _P]),
     "pal_set_wait_limit_cycles": (c_int64, [c_int64]),

@@ -743,6 +743,82 @@ int pal_paged_attention_prefill_ragged(const void* q_prompt, const void* k_promp
                         num_pages, max_pages_per_seq, scale, dtype, impl, workspace, workspace_bytes, stream);
 }
 
+size_t pal_chunk_scratch_bytes(int64_t total_tokens, int num_q_heads, int num_kv_heads, int head_dim) {
+  if (total_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_q_heads % num_kv_heads != 0) return 0;
+  return chunk_plan(total_tokens, num_q_heads, num_kv_heads, head_dim).bytes;
+}
+
+int pal_paged_attention_chunk(const void* queries, int64_t query_token_stride, int64_t query_head_stride, const void* k_pool,
+                              const void* v_pool, const void* page_table, const int32_t* sequence_lengths, const int32_t* cu_seqlens,
+                              void* out, int num_seqs, int64_t total_tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                              int tokens_per_page, int64_t num_pages, int max_pages_per_seq, float scale, int causal, int window, int dtype,
+                              void* scratch, size_t scratch_bytes, void* status, void* stream) {
+  const char* what = "paged_attention_chunk";
+  ChunkArgs a{};
+  if (!split_dtype(dtype, what, &a.dtype, &a.out_f32)) return PAL_ERR_UNSUPPORTED;
+  if (num_seqs < 0 || total_tokens < 0 || num_pages < 0 || max_pages_per_seq < 0) {
+    set_error("%s: negative sequence, token or page count", what);
+    return PAL_ERR_BAD_ARG;
+  }
+  int rc = check_heads(what, num_q_heads, num_kv_heads, head_dim, tokens_per_page);
+  if (rc != PAL_OK) return rc;
+  if (window < 0 || (window > 0 && !causal)) {
+    set_error("%s: window must not be negative, and needs causal attention", what);
+    return PAL_ERR_BAD_ARG;
+  }
+  if (total_tokens == 0 || num_seqs == 0) return PAL_OK;
+  if (!cu_seqlens && total_tokens % num_seqs != 0) {
+    set_error("%s: without cu_seqlens the number of rows must be a multiple of the number of sequences", what);
+    return PAL_ERR_BAD_ARG;
+  }
+  if (!queries || !out || !sequence_lengths || (num_pages > 0 && (!k_pool || !v_pool)) || (max_pages_per_seq > 0 && !page_table)) {
+    set_error("%s: null data pointer", what);
+    return PAL_ERR_BAD_ARG;
+  }
+  if (!aligned16(queries) || !aligned16(out) || !aligned16(k_pool) || !aligned16(v_pool) || query_token_stride % 8 != 0 ||
+      query_head_stride % 8 != 0) {
+    set_error("%s: data pointers must be 16-byte aligned and the query strides multiples of 8 elements", what);
+    return PAL_ERR_BAD_ARG;
+  }
+  // (the query strides are those of a tensor map: 40-bit byte counts; coordinates are 32-bit signed)
+  if (total_tokens > 0x7fffffffLL || num_q_heads > 0x7fffffff / head_dim || query_token_stride < 0 || query_head_stride < 0 ||
+      query_token_stride >= (1LL << 38) || query_head_stride >= (1LL << 38)) {
+    set_error("%s: token count or query strides out of range", what);
+    return PAL_ERR_BAD_ARG;
+  }
+  if (num_pages * num_kv_heads > 0x7fffffffLL / (head_dim / 8 > 0 ? head_dim / 8 : 1)) {
+    set_error("%s: pool too large (pages * kv_heads * head_dim / 8 must fit 31 bits)", what);
+    return PAL_ERR_UNSUPPORTED;
+  }
+  if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 255) || scratch_bytes < pal_chunk_scratch_bytes(total_tokens, num_q_heads, num_kv_heads, head_dim)) {
+    set_error("%s: scratch is missing, not 256-byte aligned or smaller than pal_chunk_scratch_bytes()", what);
+    return PAL_ERR_WORKSPACE;
+  }
+  a.queries = queries;
+  a.q_token_stride = query_token_stride;
+  a.q_head_stride = query_head_stride;
+  a.k_pool = k_pool;
+  a.v_pool = v_pool;
+  a.page_table = static_cast<const uint32_t*>(page_table);
+  a.seq_lens = sequence_lengths;
+  a.cu_seqlens = cu_seqlens;
+  a.out = out;
+  a.causal = causal != 0;
+  a.window = window;
+  a.num_seqs = num_seqs;
+  a.total_tokens = total_tokens;
+  a.num_q_heads = num_q_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.head_dim = head_dim;
+  a.tokens_per_page = tokens_per_page;
+  a.num_pages = max_pages_per_seq > 0 ? num_pages : 0;
+  a.max_pages_per_seq = max_pages_per_seq;
+  a.scale = scale > 0.f ? scale : 1.0f / sqrtf((float)head_dim);
+  a.status = status;
+  a.scratch = scratch;
+  return cuda_rc(launch_chunk(a, (cudaStream_t)stream), what);
+}
+
 int pal_workspace_init(void* workspace, size_t workspace_bytes, void* stream) {
   if (!workspace || workspace_bytes < sizeof(WorkspaceHeader) || (reinterpret_cast<uintptr_t>(workspace) & 255)) {
     set_error("workspace_init: a 256-byte aligned workspace of at least %zu bytes is required", sizeof(WorkspaceHeader));

@@ -1,0 +1,8 @@
+// chunk_tcgen05_kernel for head_dim = 80, tokens_per_page = 16 (a translation unit per shape keeps the build parallel).
+#include "chunk_tcgen05.cuh"
+
+namespace pal {
+
+int launch_chunk_d80_t16(const ChunkArgs& a, cudaStream_t stream) { return launch_chunk_shape<80, 16>(a, stream); }
+
+}  // namespace pal

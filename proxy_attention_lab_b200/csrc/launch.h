@@ -149,9 +149,51 @@ struct PrefillArgs {
   size_t workspace_bytes;
 };
 
+// Attention of new tokens over the paged cache alone (chunk_tcgen05.cuh).
+struct ChunkArgs {
+  const void* queries;
+  long long q_token_stride, q_head_stride;  // elements
+  const void* k_pool;
+  const void* v_pool;
+  const uint32_t* page_table;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;  // null = total_tokens / num_seqs rows per sequence
+  void* out;
+  bool out_f32;
+  bool causal;
+  int window;  // 0 = none
+  int num_seqs;
+  long long total_tokens;
+  int num_q_heads, num_kv_heads, head_dim, tokens_per_page;
+  long long num_pages;
+  int max_pages_per_seq;
+  float scale;
+  int dtype;
+  void* status;   // a word that records an expired wait (null = none)
+  void* scratch;  // chunk_plan().bytes
+};
+// An item that the border of CTA b's share cuts: its parts lie in slot 2 b + 1 and in slots 2 (b + 1), 2 (b + 2), ...
+struct ChunkCut {
+  int parts;  // 0 = none
+  int row0, tokens, head0, heads;
+};
+// What follows from the shape alone: the grid, the rows of a tile and the layout of the scratch buffer.
+struct ChunkPlan {
+  int grid;
+  int tile_heads, head_blocks, tile_tokens;
+  int part_rows;
+  size_t ml_offset, acc_offset, bytes;
+};
+// Accumulator tiles per CTA: two, or one where the O tile of head_dim 256 takes half of the tensor memory.
+constexpr int chunk_accumulators(int head_dim) { return head_dim <= 128 ? 2 : 1; }
+ChunkPlan chunk_plan(long long total_tokens, int num_q_heads, int num_kv_heads, int head_dim);
+
 // Each returns a cudaError_t value as int (0 = success) or a negative PAL_ERR_* code, and
 // leaves a message via set_error() on failure.
 int launch_fill(const FillArgs& a, cudaStream_t stream);
+int launch_chunk(const ChunkArgs& a, cudaStream_t stream);
+int launch_chunk_merge(const ChunkArgs& a, const ChunkPlan& plan, const ChunkCut* cuts, const float* part_ml, const float* part_acc,
+                       cudaStream_t stream);
 int launch_rotary(const RotaryArgs& a, cudaStream_t stream);
 int launch_decode(const DecodeArgs& a, cudaStream_t stream);
 // Strided views of a set of partial triples (element strides): partition j of row r has its m / l at

@@ -146,7 +146,8 @@ def resolve_partition_pages(partition_pages, S, hq, hkv, d, tpp, max_pages) -> i
 
 
 def check_status(stream=None, device=None) -> None:
-    """Raise ``RuntimeError`` if a kernel of the last call on this (device, stream) gave up a bounded wait.
+    """Raise ``RuntimeError`` if a kernel of the last call on this (device, stream) gave up a bounded wait, or one of any chunk
+    call on this device did.
 
     Synchronises with the stream; meant for tests and debugging."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
@@ -154,6 +155,9 @@ def check_status(stream=None, device=None) -> None:
         held = _WORKSPACES.get((device.index, sp))
         if held:
             _lib.check(lib.pal_check_status(held[-1].data_ptr(), sp))
+        page = _STATUS_PAGES.get(device.index)
+        if page is not None:
+            _lib.check(lib.pal_check_status(page.data_ptr(), sp))
 
 
 # ---------------------------------------------------------------------------------------------
@@ -826,6 +830,110 @@ def paged_attention_prefill_ragged(q_prompt, k_prompt, v_prompt, k_cache_paged, 
                                                     PREFILL_IMPL[impl] if isinstance(impl, str) else int(impl), ws.data_ptr(),
                                                     ws.numel(), sp)
         _lib.check(rc)
+    return out
+
+
+# ---------------------------------------------------------------------------------------------
+# attention of new tokens over the paged cache alone (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------------
+# device index -> a zeroed 256-byte page whose second word takes the code of an expired wait of any chunk call there
+_STATUS_PAGES: dict = {}
+
+
+def _status_page(device) -> torch.Tensor:
+    page = _STATUS_PAGES.get(device.index)
+    if page is None:
+        page = torch.zeros(256, dtype=torch.uint8, device=device)
+        # (a page that a capture creates is zeroed by the graph, not yet: later calls get one of their own)
+        if not torch.cuda.is_current_stream_capturing():
+            _STATUS_PAGES[device.index] = page
+    return page
+
+
+@functools.lru_cache(maxsize=256)
+def _chunk_scratch_bytes(device_index, total, hq, hkv, d) -> int:  # (the grid follows the device)
+    return lib.pal_chunk_scratch_bytes(total, hq, hkv, d)
+
+
+def paged_attention_chunk(queries, k_cache_pool, v_cache_pool, page_table, sequence_lengths, cu_seqlens=None, *, causal: bool = True,
+                          window=None, scale=None, out_dtype=None, out=None, stream=None):
+    """Attention of new tokens whose keys and values are already in the pages.
+
+    Sequence ``s`` owns rows ``cu_seqlens[s] .. cu_seqlens[s+1] - 1`` of ``queries [T, Hq, D]`` (``cu_seqlens [S + 1]``), or,
+    without ``cu_seqlens``, ``T / S`` rows each; ``sequence_lengths [S]`` counts all tokens of a sequence, these included.  Row
+    ``i`` of ``n`` stands at position ``L - n + i`` and sees the keys up to its own position, only the last ``window`` of them
+    when a window is given, or all ``L`` keys with ``causal=False``.  A row that sees no key becomes zeros.  Counts from a
+    single token (a decode step) to a whole prompt may be mixed; no length is read back to the host.
+
+    ``queries`` may be a strided view.  Returns ``[T, Hq, D]`` in the query dtype, or in float32 with
+    ``out_dtype=torch.float32``, written to ``out`` if given.  Rows that belong to no sequence (behind ``cu_seqlens[S]``) are
+    not written.
+    """
+    for name, t in (("queries", queries), ("k_cache_pool", k_cache_pool), ("v_cache_pool", v_cache_pool), ("page_table", page_table),
+                    ("sequence_lengths", sequence_lengths)):
+        _need_cuda(name, t)
+    if v_cache_pool.dim() != 4 or k_cache_pool.dim() != 5:
+        raise ValueError("k_cache_pool must be 5-D and v_cache_pool 4-D")
+    num_pages, hkv, d, tpp = v_cache_pool.shape
+    if tuple(k_cache_pool.shape) != (num_pages, hkv, d // 8, tpp, 8):
+        raise ValueError("k_cache_pool shape does not match v_cache_pool")
+    if not (k_cache_pool.is_contiguous() and v_cache_pool.is_contiguous()):
+        raise ValueError("the page pools must be contiguous")
+    if queries.dim() != 3 or queries.shape[2] != d:
+        raise ValueError(f"queries must be 3-D [tokens, heads, {d}], got {list(queries.shape)}")
+    if not (queries.dtype == k_cache_pool.dtype == v_cache_pool.dtype):
+        raise ValueError("queries and both pools must share one dtype")
+    code, odt = _out_code(queries.dtype, out_dtype)
+    total, hq, _ = queries.shape
+    if hq % hkv != 0:
+        raise ValueError(f"num_q_heads ({hq}) must be a multiple of num_kv_heads ({hkv})")
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be 2-D [num_sequences, max_logical_pages]")
+    S = page_table.shape[0]
+    if sequence_lengths.numel() != S:
+        raise ValueError(f"sequence_lengths must have one entry per row of page_table ({S})")
+    tensors = [("k_cache_pool", k_cache_pool), ("v_cache_pool", v_cache_pool), ("page_table", page_table), ("sequence_lengths", sequence_lengths)]
+    if cu_seqlens is not None:
+        _need_cuda("cu_seqlens", cu_seqlens)
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() != S + 1:
+            raise ValueError("cu_seqlens must hold num_sequences + 1 row offsets")
+        tensors.append(("cu_seqlens", cu_seqlens))
+    elif (S == 0 and total > 0) or (S > 0 and total % S != 0):
+        raise ValueError("without cu_seqlens the number of query rows must be a multiple of the number of sequences")
+    dev = queries.device
+    if out is not None:
+        _need_cuda("out", out)
+        if tuple(out.shape) != (total, hq, d) or out.dtype != odt or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous [{total}, {hq}, {d}] tensor of {odt}")
+        tensors.append(("out", out))
+    for name, t in tensors:
+        if t.device != dev:
+            raise ValueError(f"{name} must be on {dev}")
+    if window is not None:
+        window = int(window)
+        if window <= 0 or not causal:
+            raise ValueError("window must be positive, and needs causal attention")
+    with _Scope(dev, stream) as sp:
+        if out is None:
+            out = torch.empty((total, hq, d), dtype=odt, device=dev)
+        if total == 0 or S == 0:
+            return out
+        q = queries
+        st, sh, sd = q.stride()
+        if sd != 1 or st % 8 or sh % 8 or st <= 0 or sh <= 0 or q.data_ptr() % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+            st, sh, _ = q.stride()
+        pt = _index32("page_table", page_table)
+        lens = _index32("sequence_lengths", sequence_lengths)
+        cu = None if cu_seqlens is None else _index32("cu_seqlens", cu_seqlens)
+        # The partial results of a call live in memory of its own: calls on other streams, and captured ones, whose memory
+        # belongs to their graph, then share nothing but the status page.
+        scratch = torch.empty(_chunk_scratch_bytes(dev.index, total, hq, hkv, d), dtype=torch.uint8, device=dev)
+        status = _status_page(dev)
+        _lib.check(lib.pal_paged_attention_chunk(q.data_ptr(), st, sh, _ptr(k_cache_pool), _ptr(v_cache_pool), _ptr(pt), lens.data_ptr(),
+                                                 _ptr(cu), out.data_ptr(), S, total, hq, hkv, d, tpp, num_pages, pt.shape[1],
+                                                 0.0 if scale is None else float(scale), 1 if causal else 0, window or 0, code,
+                                                 scratch.data_ptr(), scratch.numel(), status.data_ptr() + 4, sp))
     return out
 
 

@@ -1,0 +1,286 @@
+"""paged_attention_chunk against the definition in 64 bits."""
+
+import pytest
+import torch
+
+from chunk_reference import assert_chunk, make_chunk_case
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(autouse=True)
+def short_waits(pal, cuda):
+    """A wait that cannot end gives up after a quarter of a second and fails the test."""
+    from proxy_attention_lab_b200 import _lib
+
+    before = _lib.lib.pal_set_wait_limit_cycles(500_000_000)
+    yield
+    torch.cuda.synchronize()
+    pal.check_status()
+    _lib.lib.pal_set_wait_limit_cycles(before)
+
+
+def _run(pal, case, **kw):
+    return pal.paged_attention_chunk(case["q"], case["k_pool"], case["v_pool"], case["table"], case["lens"], case["cu"],
+                                     window=case["window"], **kw)
+
+
+SHAPES = [
+    # (new tokens, lengths, hq, hkv)
+    ([1], [1], 1, 1),
+    ([1], [128], 4, 1),
+    ([1], [129], 4, 1),
+    ([5], [1000], 32, 8),
+    ([5, 1, 3, 9], [5, 700, 3, 40], 8, 2),
+    ([200], [200], 4, 2),
+    ([64, 65, 33, 1, 128], [64, 300, 33, 77, 1000], 4, 1),
+    ([300, 1, 0, 129], [700, 513, 40, 129], 6, 2),     # three heads per kv head: 126 of 128 rows used
+    ([257], [2049], 2, 2),                            # one head per kv head
+    ([40, 7], [90, 2000], 14, 2),                     # seven
+    ([3, 70], [500, 70], 40, 1),                      # forty: three tokens per tile
+    ([2, 5], [300, 5], 150, 1),                       # more heads than a tile has rows
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("new,lens,hq,hkv", SHAPES)
+def test_shapes(pal, cuda, new, lens, hq, hkv, dtype):
+    case = make_chunk_case(sum(lens), new, lens, hq, hkv, 128, dtype=dtype, device=cuda)
+    out = _run(pal, case)
+    assert out.shape == case["q"].shape and out.dtype == dtype
+    assert_chunk(out, case)
+
+
+@pytest.mark.parametrize("tpp", [16, 32])
+@pytest.mark.parametrize("d", [32, 64, 80, 96, 128, 256])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_every_instantiation(pal, cuda, d, tpp, dtype):
+    case = make_chunk_case(d + tpp, [150, 4, 1, 33], [600, 333, 1500, 33], 6, 2, d, tpp=tpp, dtype=dtype, device=cuda)
+    assert_chunk(_run(pal, case), case)
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(128, 8, 2), (64, 3, 1), (256, 4, 2)])
+def test_float32_output(pal, cuda, d, hq, hkv):
+    case = make_chunk_case(7, [90, 2], [400, 900], hq, hkv, d, dtype=BF16, device=cuda)
+    out = _run(pal, case, out_dtype=torch.float32)
+    assert out.dtype == torch.float32
+    assert_chunk(out, dict(case, out_dtype=torch.float32))
+
+
+@pytest.mark.parametrize("window", [1, 16, 100, 128, 500, 5000])
+@pytest.mark.parametrize("d,tpp", [(128, 16), (64, 32), (256, 16)])
+def test_window(pal, cuda, window, d, tpp):
+    case = make_chunk_case(window, [180, 1, 5, 64], [700, 900, 130, 64], 8, 2, d, tpp=tpp, dtype=BF16, device=cuda, window=window)
+    assert_chunk(_run(pal, case), case)
+
+
+@pytest.mark.parametrize("d", [128, 256, 32])
+def test_all_keys(pal, cuda, d):
+    case = make_chunk_case(11, [70, 1, 300], [70, 900, 555], 4, 2, d, dtype=FP16, device=cuda)
+    assert_chunk(_run(pal, case, causal=False), case, causal=False)
+
+
+def test_rows_without_keys_are_zero(pal, cuda):
+    """Lengths of zero, and lengths below the number of rows: the first rows stand before the sequence."""
+    case = make_chunk_case(12, [4, 1, 70, 3], [0, 0, 20, 1], 4, 2, 128, dtype=BF16, device=cuda)
+    out = _run(pal, case)
+    assert_chunk(out, case)
+    assert not out[:5].any() and not out[5:5 + 50].any() and out[55:75].any()
+
+
+def test_no_pages_and_no_rows(pal, cuda):
+    q = torch.randn((3, 4, 128), device=cuda).to(BF16)
+    k = torch.empty((0, 2, 16, 16, 8), dtype=BF16, device=cuda)
+    v = torch.empty((0, 2, 128, 16), dtype=BF16, device=cuda)
+    lens = torch.full((3,), 5, dtype=torch.int32, device=cuda)
+    assert not pal.paged_attention_chunk(q, k, v, torch.zeros((3, 2), dtype=torch.int32, device=cuda), lens).any()
+    assert not pal.paged_attention_chunk(q, k, v, torch.zeros((3, 0), dtype=torch.int32, device=cuda), lens).any()
+    assert pal.paged_attention_chunk(q[:0], k, v, torch.zeros((3, 2), dtype=torch.int32, device=cuda), lens).shape == (0, 4, 128)
+    empty = torch.zeros((0, 2), dtype=torch.int32, device=cuda)
+    assert pal.paged_attention_chunk(q[:0], k, v, empty, lens[:0]).shape == (0, 4, 128)
+
+
+@pytest.mark.parametrize("new,lens", [([1], [60000]), ([7], [33000]), ([1] * 3, [20000, 3, 11000]), ([200], [9000])])
+def test_long_sequences_are_cut(pal, cuda, new, lens):
+    case = make_chunk_case(13, new, lens, 8, 1, 128, dtype=BF16, device=cuda)
+    assert_chunk(_run(pal, case), case)
+
+
+def test_many_short_sequences(pal, cuda):
+    g = torch.Generator().manual_seed(14)
+    lens = torch.randint(1, 200, (700,), generator=g).tolist()
+    new = [min(L, int(n)) for L, n in zip(lens, torch.randint(0, 5, (700,), generator=g))]
+    case = make_chunk_case(14, new, lens, 4, 2, 64, dtype=FP16, device=cuda)
+    assert_chunk(_run(pal, case), case)
+
+
+def test_scale_and_large_scores(pal, cuda):
+    """Scores of hundreds: the running maximum moves, and single keys take all the weight."""
+    case = make_chunk_case(15, [100, 2], [800, 1500], 8, 2, 128, dtype=BF16, device=cuda, q_scale=20.0)
+    assert_chunk(_run(pal, case), case)
+    assert_chunk(_run(pal, case, scale=0.5), case, scale=0.5)
+
+
+def test_uniform_batches_need_no_offsets(pal, cuda):
+    case = make_chunk_case(16, [6] * 5, [6, 90, 300, 17, 1000], 8, 2, 128, dtype=BF16, device=cuda)
+    a = pal.paged_attention_chunk(case["q"], case["k_pool"], case["v_pool"], case["table"], case["lens"])
+    assert torch.equal(a.view(torch.int16), _run(pal, case).view(torch.int16))
+    assert_chunk(a, case)
+
+
+def test_rows_behind_the_last_sequence_stay(pal, cuda):
+    case = make_chunk_case(17, [5, 40], [50, 400], 4, 2, 128, dtype=BF16, device=cuda, extra_rows=9)
+    out = torch.full_like(case["q"], 7.0)
+    got = _run(pal, case, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    assert (out[45:] == 7.0).all()
+    assert_chunk(out, case)
+
+
+@pytest.mark.parametrize("kind", ["slice", "offset", "head_major", "int64"])
+def test_strided_queries_and_index_types(pal, cuda, kind):
+    case = make_chunk_case(18, [30, 2], [200, 90], 8, 2, 64, dtype=FP16, device=cuda)
+    q = case["q"]
+    if kind == "slice":
+        wide = torch.zeros((32, 12, 64), dtype=FP16, device=cuda)
+        wide[:, 2:10] = q
+        case["q"] = wide[:, 2:10]
+    elif kind == "offset":  # not 16-byte aligned: copied
+        flat = torch.zeros(q.numel() + 1, dtype=FP16, device=cuda)
+        flat[1:] = q.flatten()
+        case["q"] = flat[1:].view(q.shape)
+    elif kind == "head_major":
+        case["q"] = q.transpose(0, 1).contiguous().transpose(0, 1)
+    else:
+        for name in ("table", "lens", "cu"):
+            case[name] = case[name].long()
+    out = _run(pal, case)
+    assert out.is_contiguous()
+    assert_chunk(out, case)
+
+
+def test_repeated_calls_agree_bit_for_bit(pal, cuda):
+    case = make_chunk_case(19, [1, 300, 8, 1], [5000, 900, 2000, 64], 16, 4, 128, dtype=BF16, device=cuda)
+    first = _run(pal, case).clone()
+    for _ in range(5):
+        assert torch.equal(_run(pal, case).view(torch.int16), first.view(torch.int16))
+
+
+def test_agrees_with_decode_and_prefill(pal, cuda):
+    """One token per sequence is the decode step; a chunk is the prefill with the same keys appended first."""
+    case = make_chunk_case(20, [1] * 6, [300, 1, 2000, 17, 128, 900], 32, 8, 128, dtype=BF16, device=cuda)
+    a = _run(pal, case).float()
+    b = pal.paged_attention_decode(case["q"], case["k_pool"], case["v_pool"], case["table"], case["lens"]).float()
+    # both round P and the output to bf16: |a - b| <= 2 (eps / 2) (|v| + |out|) with |v| <= 5 over these draws
+    assert (a - b).abs().max() <= 2.0 ** -8 * 10
+    new, hist, hq, hkv, d, tpp = 70, 45, 8, 2, 128, 16
+    case = make_chunk_case(21, [new], [new + hist], hq, hkv, d, dtype=BF16, device=cuda)
+    tok = torch.arange(hist, hist + new, device=cuda)
+    page = case["table"][0].long()[tok // tpp]
+    kn = case["k_pool"][page, :, :, tok % tpp].reshape(new, hkv, d).contiguous()
+    vn = case["v_pool"][page, :, :, tok % tpp].contiguous()
+    c = pal.paged_attention_prefill(case["q"], kn, vn, case["k_pool"], case["v_pool"], case["table"],
+                                    torch.tensor([hist], dtype=torch.int32, device=cuda)).view(new, hq, d).float()
+    assert (_run(pal, case).float() - c).abs().max() <= 2.0 ** -8 * 10
+
+
+def test_two_streams_at_once(pal, cuda):
+    cases = [make_chunk_case(22 + i, [1, 50], [8000, 3000 + i], 8, 2, 128, dtype=BF16, device=cuda) for i in range(2)]
+    alone = [_run(pal, c).clone() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        outs = [_run(pal, c, stream=s) for c, s in zip(cases, streams)]
+        torch.cuda.synchronize()
+        for a, b in zip(outs, alone):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+def test_two_graphs_replayed_at_once(pal, cuda):
+    cases = [make_chunk_case(24 + i, [1, 50], [8000, 3000 + i], 8, 2, 128, dtype=BF16, device=cuda) for i in range(2)]
+    alone = [_run(pal, c).clone() for c in cases]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for c in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_run(pal, c))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, alone):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    # other lengths and queries, the same graph
+    case, graph, out = cases[0], graphs[0], outs[0]
+    case["lens"].copy_(torch.tensor([500, 50], dtype=torch.int32))
+    case["lens_list"] = [500, 50]
+    case["q"].mul_(0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert_chunk(out, case)
+
+
+def test_append_then_attend(pal, cuda):
+    """The operators as a step uses them: rotate and append the new tokens, then attend to the pages."""
+    from rotary_reference import rotate64
+
+    new, hist, hq, hkv, d, tpp = [1, 40, 3], [130, 9, 0], 8, 2, 128, 16
+    lens = [n + h for n, h in zip(new, hist)]
+    case = make_chunk_case(26, new, lens, hq, hkv, d, dtype=BF16, device=cuda, poison=False)
+    T = sum(new)
+    qkv = torch.randn((T, hq + 2 * hkv, d), generator=torch.Generator().manual_seed(1)).to(BF16)
+    pos = torch.cat([torch.arange(h, h + n) for n, h in zip(new, hist)])
+    seq = torch.cat([torch.full((n,), s) for s, n in enumerate(new)])
+    freq = (1e4 ** (-torch.arange(d // 2, dtype=torch.float64) / (d // 2))).float()
+    dq = qkv.to(cuda)
+    _, _, q = pal.fill_kv_pages_rotary(dq[:, hq:hq + hkv], dq[:, hq + hkv:], case["k_pool"], case["v_pool"], case["table"], pos.to(cuda),
+                                       seq.to(cuda), inv_freq=freq.to(cuda), queries=dq[:, :hq])
+    case["q"] = q
+    out = _run(pal, case)
+    assert_chunk(out, case)  # (the pools now hold the rotated keys)
+    page = case["table"].cpu().long()[seq, pos // tpp]
+    k = case["k_pool"].cpu()[page, :, :, pos % tpp].reshape(T, hkv, d).double()
+    assert (k - rotate64(qkv[:, hq:hq + hkv], pos, freq)).abs().max() <= 2.0 ** -8 * 8  # half a step of values below 8
+
+
+def test_refusals(pal, cuda):
+    case = make_chunk_case(27, [2, 3], [40, 50], 8, 2, 64, dtype=BF16, device=cuda)
+    q, k, v, t, l, cu = (case[n] for n in ("q", "k_pool", "v_pool", "table", "lens", "cu"))
+    call = pal.paged_attention_chunk
+    for args, kw in [
+        ((q[:, :7], k, v, t, l, cu), {}),
+        ((q[..., :32], k, v, t, l, cu), {}),
+        ((q.half(), k, v, t, l, cu), {}),
+        ((q.float(), k.float(), v.float(), t, l, cu), {}),
+        ((q[0], k, v, t, l, cu), {}),
+        ((q, k[:1], v, t, l, cu), {}),
+        ((q, k, v.transpose(2, 3), t, l, cu), {}),
+        ((q, k, v, t[0], l, cu), {}),
+        ((q, k, v, t, l[:1], cu), {}),
+        ((q, k, v, t, l, cu[:2]), {}),
+        ((q, k, v, t, l), {}),  # five rows, two sequences
+        ((q, k, v, t, l, cu), dict(window=0)),
+        ((q, k, v, t, l, cu), dict(window=-3)),
+        ((q, k, v, t, l, cu), dict(window=4, causal=False)),
+        ((q, k, v, t, l, cu), dict(out_dtype=FP16)),
+        ((q, k, v, t, l, cu), dict(out=torch.empty((5, 8, 32), dtype=BF16, device=cuda))),
+        ((q, k, v, t, l, cu), dict(out=torch.empty((5, 8, 64), device=cuda))),
+    ]:
+        with pytest.raises(ValueError):
+            call(*args, **kw)
+    with pytest.raises(TypeError):
+        call(q, k, v, t.float(), l, cu)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        call(q, k, v, t, l.cpu(), cu)
+    odd = torch.zeros((3, 2, 48, 16), dtype=BF16, device=cuda)
+    with pytest.raises(RuntimeError, match="no kernel"):
+        call(q[..., :48].contiguous(), torch.zeros((3, 2, 6, 16, 8), dtype=BF16, device=cuda), odd, t, l, cu)
