@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const Chu
     }
 #pragma unroll
     for (int sh = 16; sh >= 1; sh >>= 1) den += __shfl_xor_sync(0xffffffffu, den, sh);
-    const float inv = den > 0.f ? 1.f / den : (den == 0.f ? 0.f : den);
+    const float inv = den == 0.f ? 0.f : 1.f / den;
     const size_t o = ((size_t)(c.row0 + tok) * num_q_heads + c.head0 + head) * head_dim;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {

@@ -21,24 +21,29 @@
 // that the chain QK^T -> softmax -> PV of one tile overlaps that of the next; they are merged through shared memory at the
 // item's end (alternate).
 //
-//   warp 0      walks the CTA's share, publishes its segments in a ring in shared memory, loads Q and K
-//   warp 1      issues every tcgen05.mma and commit
-//   warp 2      loads V
+//   warp 0      walks the CTA's share, publishes its segments in a ring in shared memory, loads Q and V
+//   warp 1      issues the MMAs of S = Q K^T, warp 2 those of O += P V
+//   warp 3      loads K
 //   warps 4..   one softmax warpgroup per accumulator: thread = row = TMEM lane
 //
 // Operand layouts are those of the prefill kernel (prefill_tcgen05.cuh): Q K-major with the 128-byte swizzle; a key tile
-// gathered chunk by chunk from the pages as [D/8][128 tokens][16 B], K-major without swizzle; V pages [D][TPP] K-major with
-// the 32- or 64-byte swizzle.  TMEM: S tiles of 128 columns (P overwrites its S tile's first 64; the residual of P, where it
-// is fed, the other 64), then O tiles of D columns.  head_dim 256 leaves room for one O tile only: one accumulator with S
-// double-buffered.
+// copied chunk by chunk from the pages as [D/8][128 tokens][16 B], K-major without swizzle; V pages [D][TPP] K-major with
+// the 32- or 64-byte swizzle.
+//
+// TMEM: a buffer of 128 fp32 scores (two for head_dim <= 64), a P tile of 64 columns per accumulator, the O tiles.  P does not
+// overwrite the scores: the softmax warps hold a whole row of them in registers, so the score buffer is free after one read
+// and takes the next QK^T, of the other accumulator, while the exponentials are computed.  (With P over S, as the prefill kernel
+// has it, softmax, PV and the next QK^T of an accumulator form a chain: 4270 cycles per 2 x 128 x 128 scores at head_dim 128.)
 #pragma once
+
+#include <type_traits>
 
 #include "prefill_tcgen05.cuh"
 
 namespace pal {
 namespace {
 
-constexpr int kChunkItemCost = 2;    // fixed cost of an item in key tiles: query load, pipeline fill, epilogue
+constexpr int kChunkItemCost = 6;    // fixed cost of an item in key tiles: query load, pipeline fill, epilogue
 constexpr int kChunkMinShare = 4;    // smallest share of a CTA, in the same unit
 constexpr int kSegRing = 4;
 
@@ -57,6 +62,7 @@ struct ChunkSegment {
 };
 
 struct ChunkParams {
+  const void* k_pool;
   const uint32_t* page_table;
   const int32_t* seq_lens;
   const int32_t* cu_seqlens;  // null = every sequence has tokens_per_seq rows
@@ -110,15 +116,21 @@ __device__ __forceinline__ int chunk_keys(const ChunkParams& p, const ChunkSeq& 
 
 template <int D_, int TPP_, int NQ_>
 struct ChunkCfg {
-  static constexpr int D = D_, TPP = TPP_, NQ = NQ_, SBUF = NQ == 1 ? 2 : 1;
-  using Base = TcCfg<D, TPP, NQ, SBUF>;
+  static constexpr int D = D_, TPP = TPP_, NQ = NQ_;
+  using Base = TcCfg<D, TPP, NQ, 1>;  // operand tile sizes and ring depth
+  // TMEM columns: S buffers (128 fp32 scores), a P tile per accumulator (128 weights, two to a column), O tiles
+  static constexpr int kSBuffers = D <= 64 ? 2 : 1;
+  static constexpr int kPCol = kSBuffers * kTile;
+  static constexpr int kOCol = kPCol + NQ * 64;
+  static_assert(kOCol + NQ * Base::DP <= 512, "TMEM holds 512 columns");
   static constexpr int kThreads = 128 + 128 * NQ;
   static constexpr int ST = Base::kStages;
   static constexpr int kQ = 0;
   static constexpr int kK = NQ * Base::kTileBytes;
   static constexpr int kV = kK + ST * Base::kTileBytes;
   static constexpr int kMl = kV + ST * Base::kTileBytes;    // m, l of the second accumulator (alternate segments)
-  static constexpr int kBars = kMl + (NQ == 2 ? 1024 : 0);
+  static constexpr int kStage = kMl + (NQ == 2 ? 1024 : 0);  // 4 KB per softmax warp on the way out
+  static constexpr int kBars = kStage + NQ * 4 * 4096;
   static constexpr int kUsed = kBars + 512 + kSegRing * (int)sizeof(ChunkSegment) + 1024;
   static constexpr int kTotal = kUsed < 116 * 1024 ? 116 * 1024 : kUsed;
   // the second Q tile as a buffer of fp32 rows: 16-byte pieces per row (whole groups of eight) and rows that fit
@@ -126,6 +138,36 @@ struct ChunkCfg {
   static constexpr int kMergeRows = Base::kTileBytes / (16 * kMergePitch) < 128 ? 64 : 128;
   static_assert(kMergeRows * kMergePitch * 16 <= Base::kTileBytes, "merge buffer");
 };
+
+// Has the phase completed?  Never suspends the thread (mbar_try_wait may, for microseconds).
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// tcgen05.mma with operand descriptors given as (lower, upper) halves; `accumulate` 0 starts the accumulator afresh.
+__device__ __forceinline__ void tc_mma_ss32(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %6, 0;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts32(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 
 // Row maximum of 128 scores in registers: eight chains.
 __device__ __forceinline__ float row_max128(const uint32_t (&s)[128]) {
@@ -151,40 +193,64 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&s)[128]) {
   tmem_ld32(taddr + 96, d);
 }
 
-// P = exp2(s * scale - m_ref) of one row, rounded to the input type and packed over the S tile's first 64 columns; the
-// rounding residual, where it is fed, over the other 64.  The row sum is taken before the rounding.
+// P = exp2(s * scale - m_ref) of keys 64 h .. 64 h + 63 of one row, rounded to the input type, two keys to a register.  The
+// row sum is taken before the rounding.  The special-function unit (16 per clock) needs 1024 cycles for the 128 x 128
+// exponentials of a tile, as long as the tile's MMAs keep the tensor pipe.  (A part of them on the FMA pipe, as a polynomial of
+// degree 3, was measured: one in eight gains 4 % of the cycles and nothing of the time, the clock gives way to the power limit;
+// one in four or more loses.)
 template <typename T>
-__device__ __forceinline__ void chunk_exp_store(uint32_t tS, const uint32_t (&s)[128], float scale_log2, float m_ref, bool residual, float& l_run) {
-  using PK = Mma16816<T>;
-  float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+__device__ __forceinline__ void chunk_exp_half(const uint32_t (&s)[128], int h, float scale_log2, float m_ref, uint32_t (&out)[32], float2 (&acc)[2]) {
   const float2 sc2 = make_float2(scale_log2, scale_log2), nm2 = make_float2(-m_ref, -m_ref);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t hi[32];
-    if (PK::kSplitP && residual) {
-      uint32_t lo[32];
-#pragma unroll
-      for (int w = 0; w < 32; ++w) {
-        const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[64 * h + 2 * w]), __uint_as_float(s[64 * h + 2 * w + 1])), sc2, nm2);
-        const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-        hi[w] = PK::pack(e.x, e.y);
-        lo[w] = PK::pack_residual(e.x, e.y, hi[w]);
-        acc[w & 1] = __fadd2_rn(acc[w & 1], e);
-      }
-      tmem_st32(tS + 64 + 32 * h, lo);
-    } else {
-#pragma unroll
-      for (int w = 0; w < 32; ++w) {
-        const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[64 * h + 2 * w]), __uint_as_float(s[64 * h + 2 * w + 1])), sc2, nm2);
-        const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-        hi[w] = PK::pack(e.x, e.y);
-        acc[w & 1] = __fadd2_rn(acc[w & 1], e);
-      }
-    }
-    tmem_st32(tS + 32 * h, hi);
+  for (int w = 0; w < 32; ++w) {
+    const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[64 * h + 2 * w]), __uint_as_float(s[64 * h + 2 * w + 1])), sc2, nm2);
+    const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+    out[w] = Mma16816<T>::pack(e.x, e.y);
+    acc[w & 1] = __fadd2_rn(acc[w & 1], e);
   }
-  l_run += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
 }
+
+// Items that feed the rounding residual take a path of their own, in rolled loops of 32 columns over the scores in place.
+// Maximum over the columns in [lo, hi]:
+__device__ __forceinline__ float chunk_residual_max(uint32_t tS, int lo, int hi) {
+  float m = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < kTile; c += 32) {
+    uint32_t v[32];
+    tmem_ld32(tS + c, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (c + i >= lo && c + i <= hi) m = fmaxf(m, __uint_as_float(v[i]));
+  }
+  return m;
+}
+// ... and P: zero outside, the residual over the first 64 columns of the scores (never ahead of those still to be read).
+// Returns the row sum.
+template <typename T>
+__device__ __forceinline__ float chunk_residual_exp(uint32_t tS, uint32_t tP, int lo, int hi, float scale_log2, float m_ref) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < kTile; c += 32) {
+    uint32_t v[32], w[16], r[16];
+    tmem_ld32(tS + c, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float a = c + i >= lo && c + i <= hi ? fast_exp2(fmaf(__uint_as_float(v[i]), scale_log2, -m_ref)) : 0.f;
+      const float b = c + i + 1 >= lo && c + i + 1 <= hi ? fast_exp2(fmaf(__uint_as_float(v[i + 1]), scale_log2, -m_ref)) : 0.f;
+      w[i / 2] = Mma16816<T>::pack(a, b);
+      r[i / 2] = Mma16816<T>::pack_residual(a, b, w[i / 2]);
+      sum += a + b;
+    }
+    tmem_st16(tP + c / 2, w);
+    tmem_st16(tS + c / 2, r);
+  }
+  return sum;
+}
+
+// 1 / l for the row sum l: 0 for a row without keys, NaN where a score was not a number
+__device__ __forceinline__ float chunk_inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 // bf16 rounds P by up to 2^-9 of its value, which leaves about 0.002 / sqrt(n / 3) per unit of |v| over n keys.  Items with a
 // row of fewer than 256 keys, and float32 outputs, get the residual P - bf16(P) through a second set of PV MMAs.
@@ -196,13 +262,45 @@ __device__ __forceinline__ bool chunk_feeds_residual(const ChunkParams& p, const
   return p.out_f32 != 0 || keys < 256;
 }
 
+// The 32 rows of a warp, one per lane in registers, to rows `row` (-1 = none) of `base` by way of `stage` (128 bytes per row):
+// written as they are held, an instruction would write 16 bytes of 32 rows; from shared memory it writes contiguous bytes of a
+// few.  EB = bytes per element; columns(c, x) gives columns [c * OC, (c + 1) * OC), pack(x) makes 16 bytes of them.
+template <int D, int OC, int EB, typename Columns, typename Pack>
+__device__ __forceinline__ void chunk_store_rows(unsigned char* stage, int lane, unsigned char* base, int row, const Columns& columns, const Pack& pack) {
+  constexpr int kPieces = OC * EB / 16;  // 2, 4 or 8
+  int to[kPieces];
+#pragma unroll
+  for (int it = 0; it < kPieces; ++it) to[it] = __shfl_sync(0xffffffffu, row, (it * 32 + lane) / kPieces);
+  constexpr int kUnroll = EB == 2 && D / OC <= 2 ? 2 : 1;  // (the usual output goes straight through; the others are rolled)
+#pragma unroll kUnroll
+  for (int c = 0; c < D / OC; ++c) {
+    float x[OC];
+    columns(c, x);
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) *reinterpret_cast<uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4)) = pack(x + k * (16 / EB));
+    __syncwarp();
+    uint4 v[kPieces];
+#pragma unroll
+    for (int it = 0; it < kPieces; ++it) {
+      const int r = (it * 32 + lane) / kPieces, piece = (it * 32 + lane) % kPieces;
+      v[it] = *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+    }
+#pragma unroll
+    for (int it = 0; it < kPieces; ++it) {
+      const int piece = (it * 32 + lane) % kPieces;
+      if (to[it] >= 0) *reinterpret_cast<uint4*>(base + (size_t)to[it] * (D * EB) + (c * kPieces + piece) * 16) = v[it];
+    }
+    __syncwarp();
+  }
+}
+
 template <typename T, int D, int TPP, int NQ>
 __global__ void __launch_bounds__(128 + 128 * NQ, 1)
     chunk_tcgen05_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap tm_q,
-                         const __grid_constant__ CUtensorMap tm_kpool, const __grid_constant__ CUtensorMap tm_vpool) {
+                         const __grid_constant__ CUtensorMap tm_vpool) {
   using C = ChunkCfg<D, TPP, NQ>;
   using B = typename C::Base;
-  constexpr int ST = C::ST, SBUF = C::SBUF, kThreadsAll = C::kThreads;
+  constexpr int ST = C::ST, NS = C::kSBuffers, kThreadsAll = C::kThreads;
   constexpr int kBlocks = B::kBlocks, kPagesPerTile = B::kPagesPerTile, kPageBytes = B::kPageBytes, kTileBytes = B::kTileBytes;
   constexpr int kOC = B::kOChunk;
   extern __shared__ unsigned char smem_raw[];
@@ -218,16 +316,17 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
   uint64_t* k_empty = bars + 4;        // ST
   uint64_t* v_full = bars + 6;         // ST
   uint64_t* v_empty = bars + 8;        // ST
-  uint64_t* s_full = bars + 10;        // 2: per accumulator, or per S buffer
-  uint64_t* p_full = bars + 12;        // 2
-  uint64_t* o_done = bars + 14;        // 2: last PV of a segment (NQ = 2), every PV (NQ = 1)
+  uint64_t* s_full = bars + 10;        // 2, per accumulator: its scores are in an S buffer
+  uint64_t* s_empty = bars + 28;       // 2: ... and have been read
+  uint64_t* p_full = bars + 12;        // 2: its P tile is written
+  uint64_t* o_done = bars + 14;        // 2: the PV that read it has run
   uint64_t* merge_full = bars + 16;    // 1: the second accumulator's rows are in shared memory
   uint64_t* merge_empty = bars + 17;   // 1
   uint64_t* seg_done = bars + 18;      // 1: the first warpgroup has finished a segment
   uint64_t* seg_full = bars + 20;      // kSegRing
   uint64_t* seg_empty = bars + 24;     // kSegRing
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 30);
-  long long* sm_plan = reinterpret_cast<long long*>(bars + 32);  // scan scratch, then the share's first item
+  long long* sm_plan = reinterpret_cast<long long*>(bars + 32);  // scan scratch, then the share's last item
   ChunkSegment* segs = reinterpret_cast<ChunkSegment*>(smem + C::kBars + 512);
   static_assert(kSegRing == 4, "barrier layout");
 
@@ -260,12 +359,13 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       mbar_init(q_full, 1);
       mbar_init(q_empty, 1);
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&k_full[i], 1);
+        mbar_init(&k_full[i], 32);
         mbar_init(&k_empty[i], 1);
         mbar_init(&v_full[i], 1);
         mbar_init(&v_empty[i], 1);
         mbar_init(&s_full[i], 1);
         mbar_init(&p_full[i], 4);
+        mbar_init(&s_empty[i], 4);
         mbar_init(&o_done[i], 1);
       }
       mbar_init(merge_full, 4);
@@ -273,7 +373,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       mbar_init(seg_done, 4);
       for (int i = 0; i < kSegRing; ++i) {
         mbar_init(&seg_full[i], 1);
-        mbar_init(&seg_empty[i], 2 + 4 * NQ);
+        mbar_init(&seg_empty[i], 3 + 4 * NQ);
       }
       fence_mbar_init();
     }
@@ -296,8 +396,9 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
     share1 = min(share0 + share, total);
     __syncthreads();
     const long long start = before + inc - mine;
-    if (share0 < share1 && share0 >= start && share0 < start + mine) {
-      // the share begins in this thread's run: find the item
+    const long long last = share1 - 1;
+    if (share0 < share1 && last >= start && last < start + mine) {
+      // the share ends in this thread's run: find the item
       long long at = start;
       int s = sa, vh = 0, ta = 0;
       for (; s < sb; ++s) {
@@ -305,12 +406,12 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
         long long w = 0;
         int lo, hi;
         for (int t = 0; t < q.n; t += item_tokens) w += kChunkItemCost + chunk_keys(p, q, t, min(t + item_tokens, q.n), lo, hi);
-        if (share0 < at + w * vheads) {
-          vh = (int)((share0 - at) / w);
+        if (last < at + w * vheads) {
+          vh = (int)((last - at) / w);
           at += vh * w;
           for (;; ta += item_tokens) {
             const int c = kChunkItemCost + chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi);
-            if (share0 < at + c) break;
+            if (last < at + c) break;
             at += c;
           }
           break;
@@ -334,13 +435,17 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
   if (warp < 4) {
   if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == 0) {
-    // =============================== segments, Q and K ===============================
+    // =============================== segments, Q and V ===============================
     if (share0 >= share1) {
       if (lane == 0) p.cuts[blockIdx.x].parts = 0;
     }
+    // The share is walked backwards.  What it holds of its last item are that item's first keys, and what it holds of its
+    // first item that item's last ones: so all CTAs start at the first keys and end at the last, and row tiles of one head,
+    // which lie on neighbouring CTAs, read the same pages at about the same time (from L2, when one sequence is larger).
     int s = 0, vh = 0, ta = 0;
-    long long at = share0, share = 1;
-    if (share0 < share1) {
+    long long at = 0, share = 1;  // at: where the current item starts
+    bool more = share0 < share1;
+    if (more) {
       s = (int)sm_plan[0];
       vh = (int)sm_plan[1];
       ta = (int)sm_plan[2];
@@ -348,341 +453,286 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       share = sm_plan[4];
     }
     __syncwarp();
-    ChunkSeq q = share0 < share1 ? chunk_seq(p, s, TPP) : ChunkSeq{};
-    uint32_t n_seg = 0, n_tile = 0;  // segments and key tiles so far (ring positions)
-    bool prev_alternate = false;
+    ChunkSeq q = more ? chunk_seq(p, s, TPP) : ChunkSeq{};
+    int lo = 0, hi = 0, nt = more ? chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi) : 0;
+    uint32_t n_pub = 0;  // segments published (ring position)
     bool cut_written = false;
-    int ok = 1;
-    while (ok) {
+    // next segment of the share (the same computation on every lane), published to the other warps
+    auto publish = [&]() {
       // ---- next segment of the share (the same computation on every lane) ----
       ChunkSegment g;
       g.end = 1;
-      while (at < share1) {
-        const int tb = min(ta + item_tokens, q.n);
-        int lo = 0, hi = 0, nt = 0, cost = 0;
-        if (q.n > 0) {
-          nt = chunk_keys(p, q, ta, tb, lo, hi);
-          cost = kChunkItemCost + nt;
-          const long long first = at + kChunkItemCost;  // place of key tile 0 on the line
-          const int t0 = (int)min((long long)nt, max(0LL, share0 - first)), t1 = (int)max(0LL, min((long long)nt, share1 - first));
-          if (t1 > t0 || (nt == 0 && at >= share0)) {
-            g.end = 0;
-            g.seq = s;
-            g.kv_head = vh / p.head_blocks;
-            const int hb = vh - g.kv_head * p.head_blocks;
-            g.head0 = g.kv_head * p.group + hb * p.tile_heads;
-            g.heads = min(p.tile_heads, p.group - hb * p.tile_heads);
-            g.row0 = q.row0 + ta;
-            g.tokens = tb - ta;
-            g.pos0 = q.len - q.n + ta;
-            g.kt0 = lo / kTile + t0;
-            g.kt1 = lo / kTile + t1;
-            g.key_lo = lo;
-            g.key_hi = hi;
-            g.key_cap = q.cap;
-            g.alternate = NQ == 2 && g.tokens <= p.tile_tokens;
-            g.slot = t0 > 0 ? 2 * (int)blockIdx.x : (t1 < nt ? 2 * (int)blockIdx.x + 1 : -1);
-            if (t0 == 0 && t1 < nt && lane == 0) {
-              // this CTA holds the item's first part: tell the merging kernel where the others are
-              ChunkCut c;
-              c.parts = (int)((first + nt - 1) / share) - (int)blockIdx.x + 1;
-              c.row0 = g.row0;
-              c.tokens = g.tokens;
-              c.head0 = g.head0;
-              c.heads = g.heads;
-              p.cuts[blockIdx.x] = c;
-              cut_written = true;
-            }
+      while (more && g.end) {
+        const long long first = at + kChunkItemCost;  // place of key tile 0 on the line
+        const int t0 = (int)min((long long)nt, max(0LL, share0 - first)), t1 = (int)max(0LL, min((long long)nt, share1 - first));
+        if (t1 > t0 || (nt == 0 && at >= share0)) {
+          g.end = 0;
+          g.seq = s;
+          g.kv_head = vh / p.head_blocks;
+          const int hb = vh - g.kv_head * p.head_blocks;
+          g.head0 = g.kv_head * p.group + hb * p.tile_heads;
+          g.heads = min(p.tile_heads, p.group - hb * p.tile_heads);
+          g.row0 = q.row0 + ta;
+          g.tokens = min(item_tokens, q.n - ta);
+          g.pos0 = q.len - q.n + ta;
+          g.kt0 = lo / kTile + t0;
+          g.kt1 = lo / kTile + t1;
+          g.key_lo = lo;
+          g.key_hi = hi;
+          g.key_cap = q.cap;
+          g.alternate = NQ == 2 && g.tokens <= p.tile_tokens;
+          g.slot = t0 > 0 ? 2 * (int)blockIdx.x : (t1 < nt ? 2 * (int)blockIdx.x + 1 : -1);
+          if (t0 == 0 && t1 < nt && lane == 0) {
+            // this CTA holds the item's first part: tell the merging kernel where the others are
+            ChunkCut c;
+            c.parts = (int)((first + nt - 1) / share) - (int)blockIdx.x + 1;
+            c.row0 = g.row0;
+            c.tokens = g.tokens;
+            c.head0 = g.head0;
+            c.heads = g.heads;
+            p.cuts[blockIdx.x] = c;
+            cut_written = true;
           }
         }
-        // advance: row tiles, then heads, then sequences
-        at += cost;
-        ta += item_tokens;
-        if (ta >= q.n) {
-          ta = 0;
-          if (q.n <= 0 || ++vh == vheads) {
-            vh = 0;
-            ++s;
-            if (at < share1) q = chunk_seq(p, s, TPP);
-          }
-        }
-        if (!g.end) break;
-      }
-      // ---- publish it ----
-      const int slot = n_seg % kSegRing;
-      if (lane == 0) {
-        ok = mbar_wait(&seg_empty[slot], ((n_seg / kSegRing) & 1) ^ 1, p.status);
-        if (ok) {
-          segs[slot] = g;
-          mbar_arrive(&seg_full[slot]);
-        }
-      }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (!ok || g.end) break;
-      if (g.kt0 < g.kt1) {
-        // ---- Q: free once the last QK^T of the previous segment with keys has run; the second tile also serves as the
-        // merge buffer of alternate segments ----
-        if (lane == 0) {
-          ok = mbar_wait(q_empty, (n_seg & 1) ^ 1, p.status);
-          if (ok && !g.alternate && prev_alternate) ok = mbar_wait(seg_done, (n_seg & 1) ^ 1, p.status);
-          if (ok) {
-            const int tiles = NQ == 2 && !g.alternate ? 2 : 1;
-            mbar_arrive_expect_tx(q_full, tiles * kBlocks * p.tile_heads * p.tile_tokens * 128);
-            for (int t = 0; t < tiles; ++t)
-              for (int kb = 0; kb < kBlocks; ++kb)
-                tma_load_3d(sQ + t * kTileBytes + kb * kBlockBytes, &tm_q, kb * 64, g.head0, g.row0 + t * p.tile_tokens, q_full);
-          }
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-      } else if (lane == 0) {
-        // no keys: the segment passes through the barriers that count segments
-        ok = mbar_wait(q_empty, (n_seg & 1) ^ 1, p.status);
-        if (ok) mbar_arrive(q_full);
-      }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      prev_alternate = g.alternate != 0;
-      ++n_seg;
-      // ---- K ----
-      const uint32_t* pages = p.page_table + (size_t)g.seq * p.max_pages_per_seq;
-      for (int j = g.kt0; j < g.kt1 && ok; ++j, ++n_tile) {
-        const int st = n_tile % ST;
-        // pages [pg0, pg1) of the tile hold visible keys; the others are not fetched (their columns of S are masked)
-        const int pg0 = max(0, g.key_lo - j * kTile) / TPP;
-        const int pg1 = (min(kTile, g.key_hi - j * kTile) + TPP - 1) / TPP;
-        uint32_t pid = 0;
-        if (lane < kPagesPerTile) {
-          pid = pages[j * kPagesPerTile + min(max(lane, pg0), pg1 - 1)];
-          if ((long long)pid >= p.num_pages) pid = (uint32_t)(p.num_pages - 1);
-        }
-        if (lane == 0) ok = mbar_wait(&k_empty[st], ((n_tile / ST) & 1) ^ 1, p.status);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) break;
-        constexpr int kChunks = D / 8, kGroups = kPagesPerTile / 4;
-        constexpr int kGroupBytes = 4 * TPP * 16;
-        const int g0 = pg0 >> 2, g1 = (pg1 + 3) >> 2;
-        if (lane == 0) mbar_arrive_expect_tx(&k_full[st], kChunks * (g1 - g0) * kGroupBytes);
-        __syncwarp();
-#pragma unroll
-        for (int op0 = 0; op0 < kChunks * kGroups; op0 += 32) {
-          const int op = op0 + lane;
-          const int c = op / kGroups, gr = op % kGroups;
-          int rows[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) rows[i] = ((int)__shfl_sync(0xffffffffu, pid, (4 * gr + i) & 31) * p.num_kv_heads + g.kv_head) * kChunks + c;
-          if (op < kChunks * kGroups && gr >= g0 && gr < g1)
-            tma_gather4(sK + st * kTileBytes + c * B::kChunkBytes + gr * kGroupBytes, &tm_kpool, 0, rows[0], rows[1], rows[2], rows[3],
-                        &k_full[st]);
-        }
-      }
-    }
-    if (lane == 0 && share0 < share1 && !cut_written) p.cuts[blockIdx.x].parts = 0;
-  } else if (warp == 1) {
-    // =============================== MMA issuer ===============================
-    constexpr int F = Fmt<T>::kCode;
-    constexpr uint32_t idesc_qk = make_idesc(128, F, F, 0);
-    constexpr uint32_t idesc_pv = make_idesc(D, F, F, 0);
-    const uint64_t q_desc = make_desc(smem_u32(sQ), 16, 1024, kLayoutSw128);
-    const uint64_t k_desc = make_desc(smem_u32(sK), B::kChunkBytes, 128, kLayoutNone);
-    const uint64_t v_desc = make_desc(smem_u32(sV), 16, 8 * TPP * 2, TPP == 16 ? kLayoutSw32 : kLayoutSw64);
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)) != 0; };
-    uint32_t n_seg = 0, kt = 0, vt = 0;  // segments, key tiles whose QK^T / PV have been issued
-    uint32_t n_p0 = 0, n_p1 = 0;         // P tiles taken from each accumulator (NQ = 2)
-    bool ok = true;
-    // S(si) = Q(tile) . K^T of the next key tile
-    auto issue_qk = [&](int q_tile, int si, int st) {
-      if (!elect_one()) return;
-      const uint32_t d_tmem = tmem_base + si * kTile;
-      const uint64_t qa = q_desc + (uint64_t)(q_tile * (kTileBytes >> 4)), kb = k_desc + (uint64_t)(st * (kTileBytes >> 4));
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks)
-        tc_mma_ss(d_tmem, qa + (uint64_t)(((ks >> 2) * kBlockBytes + (ks & 3) * 32) >> 4), kb + (uint64_t)((ks * 2 * B::kChunkBytes) >> 4), idesc_qk,
-                  ks > 0);
-      tc_commit(&s_full[si]);
-    };
-    // O(acc) += P(si) . V over the 16-key steps [kk0, kk1); `first`: the accumulator starts afresh
-    auto issue_pv = [&](int acc, int si, int st, int kk0, int kk1, bool first, bool residual) {
-      if (!elect_one()) return;
-      const uint32_t d_tmem = tmem_base + B::kOBase + acc * B::DP;
-      const uint64_t vb = v_desc + (uint64_t)(st * (kTileBytes >> 4));
-      uint32_t accumulate = first ? 0u : 1u;
-      for (int part = 0; part < (residual ? 2 : 1); ++part) {
-        const uint32_t a_tmem = tmem_base + si * kTile + part * 64;
-        if (kk0 == 0 && kk1 == kTile / 16) {
-#pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk) {
-            const int off = TPP == 16 ? kk * kPageBytes : (kk >> 1) * kPageBytes + (kk & 1) * 32;
-            tc_mma_ts(d_tmem, a_tmem + kk * 8, vb + (uint64_t)(off >> 4), idesc_pv, accumulate);
-            accumulate = 1u;
-          }
+        // back to the item before, if the share reaches it: row tiles, then heads, then sequences
+        more = at > share0;
+        if (!more) break;
+        if (ta > 0) {
+          ta -= item_tokens;
         } else {
-#pragma unroll 1
-          for (int kk = kk0; kk < kk1; ++kk) {
-            const int off = TPP == 16 ? kk * kPageBytes : (kk >> 1) * kPageBytes + (kk & 1) * 32;
-            tc_mma_ts(d_tmem, a_tmem + kk * 8, vb + (uint64_t)(off >> 4), idesc_pv, accumulate);
-            accumulate = 1u;
+          if (--vh < 0) {
+            vh = vheads - 1;
+            do q = chunk_seq(p, --s, TPP);
+            while (q.n <= 0);  // (an item lies before this one: at > 0)
           }
+          ta = (q.n - 1) / item_tokens * item_tokens;
         }
+        nt = chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi);
+        at -= kChunkItemCost + nt;
       }
+      const int slot = n_pub % kSegRing;
+      if (!__all_sync(0xffffffffu, mbar_wait(&seg_empty[slot], ((n_pub / kSegRing) & 1) ^ 1, p.status))) return false;
+      if (lane == 0) {
+        segs[slot] = g;
+        mbar_arrive(&seg_full[slot]);
+      }
+      __syncwarp();
+      ++n_pub;
+      return true;
     };
-    auto commit = [&](uint64_t* bar) {
-      if (elect_one()) tc_commit(bar);
-    };
-    while (ok) {
-      const int slot = n_seg % kSegRing;
-      ok = wait_all(&seg_full[slot], (n_seg / kSegRing) & 1);
-      if (!ok) break;
-      const ChunkSegment g = segs[slot];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&seg_empty[slot]);
-      if (g.end) break;
-      ok = wait_all(q_full, n_seg & 1);
-      ++n_seg;
-      if (!ok) break;
-      if (g.kt0 >= g.kt1) {
-        if (lane == 0) mbar_arrive(q_empty);
-        continue;
-      }
-      const bool residual = chunk_feeds_residual<T>(p, g);
-      const int num = g.kt1 - g.kt0;
-      auto steps = [&](int j, int& kk0, int& kk1) {
-        kk0 = max(0, g.key_lo - j * kTile) >> 4;
-        kk1 = (min(kTile, g.key_hi - j * kTile) + 15) >> 4;
-      };
-      auto wait_k = [&]() {
-        const bool r = wait_all(&k_full[kt % ST], (kt / ST) & 1);
-        tc_fence_after();
-        return r;
-      };
-      auto wait_v = [&]() { return wait_all(&v_full[vt % ST], (vt / ST) & 1); };
-      auto wait_p = [&](int si) {
-        const uint32_t n = NQ == 1 ? vt >> 1 : (si ? n_p1++ : n_p0++);  // (the two S buffers of one accumulator take turns)
-        const bool r = wait_all(&p_full[si], n & 1);
-        tc_fence_after();
-        return r;
-      };
-      int kk0, kk1;
-      if (NQ == 1) {
-        // one accumulator, two S buffers: QK^T of tile i + 1 runs under the softmax of tile i
-        ok = wait_k();
-        if (!ok) break;
-        issue_qk(0, kt & 1, kt % ST);
-        commit(&k_empty[kt % ST]);
-        ++kt;
-        if (num == 1) commit(q_empty);
-        for (int i = 0; i < num && ok; ++i) {
-          if (i + 1 < num) {
-            ok = wait_k();
-            if (!ok) break;
-            issue_qk(0, kt & 1, kt % ST);
-            commit(&k_empty[kt % ST]);
-            ++kt;
-            if (i + 2 == num) commit(q_empty);
-          }
-          const int si = vt & 1;
-          ok = wait_v() && wait_p(si);
-          if (!ok) break;
-          steps(g.kt0 + i, kk0, kk1);
-          issue_pv(0, si, vt % ST, kk0, kk1, i == 0, residual);
-          commit(&o_done[si]);
-          commit(&v_empty[vt % ST]);
-          ++vt;
-        }
-      } else if (g.alternate) {
-        for (int i = 0; i < 2 && i < num && ok; ++i) {
-          ok = wait_k();
-          if (!ok) break;
-          issue_qk(0, i, kt % ST);
-          commit(&k_empty[kt % ST]);
-          ++kt;
-        }
-        if (ok && num <= 2) commit(q_empty);
-        for (int i = 0; i < num && ok; ++i) {
-          const int a = i & 1;
-          ok = wait_v() && wait_p(a);
-          if (!ok) break;
-          steps(g.kt0 + i, kk0, kk1);
-          issue_pv(a, a, vt % ST, kk0, kk1, i < 2, residual);
-          commit(&v_empty[vt % ST]);
-          ++vt;
-          if (i + 2 < num) {
-            ok = wait_k();
-            if (!ok) break;
-            issue_qk(0, a, kt % ST);
-            commit(&k_empty[kt % ST]);
-            ++kt;
-            if (i + 3 == num) commit(q_empty);
-          } else {
-            commit(&o_done[a]);
-          }
-        }
-      } else {
-        ok = wait_k();
-        if (!ok) break;
-        issue_qk(0, 0, kt % ST);
-        issue_qk(1, 1, kt % ST);
-        commit(&k_empty[kt % ST]);
-        ++kt;
-        if (num == 1) commit(q_empty);
-        for (int i = 0; i < num && ok; ++i) {
-          ok = wait_v();
-          steps(g.kt0 + i, kk0, kk1);
-          for (int a = 0; a < 2 && ok; ++a) {
-            ok = wait_p(a);
-            if (!ok) break;
-            issue_pv(a, a, vt % ST, kk0, kk1, i == 0, residual);
-            if (i + 1 < num) {
-              if (a == 0) ok = wait_k();
-              if (!ok) break;
-              issue_qk(a, a, kt % ST);
-            } else {
-              commit(&o_done[a]);
-            }
-          }
-          if (!ok) break;
-          commit(&v_empty[vt % ST]);
-          ++vt;
-          if (i + 1 < num) {
-            commit(&k_empty[kt % ST]);
-            ++kt;
-            if (i + 2 == num) commit(q_empty);
-          }
+    uint32_t n_tile = 0;
+    bool prev_alternate = false;
+    int ok = publish();
+    for (uint32_t n_seg = 0; ok; ++n_seg) {
+      const ChunkSegment& g = segs[n_seg % kSegRing];  // (not overwritten before three more are published)
+      const int end = g.end, kt0 = g.kt0, kt1 = g.kt1, alternate = g.alternate;
+      if (end) break;
+      // ---- Q: free once the last QK^T of the previous segment has run; the second tile also serves as the merge buffer of
+      // alternate segments ----
+      if (lane == 0) {
+        ok = mbar_wait(q_empty, (n_seg & 1) ^ 1, p.status);
+        if (ok && !alternate && prev_alternate) ok = mbar_wait(seg_done, (n_seg & 1) ^ 1, p.status);
+        if (ok && kt0 < kt1) {
+          const int tiles = NQ == 2 && !alternate ? 2 : 1;
+          mbar_arrive_expect_tx(q_full, tiles * kBlocks * p.tile_heads * p.tile_tokens * 128);
+          for (int t = 0; t < tiles; ++t)
+            for (int kb = 0; kb < kBlocks; ++kb)
+              tma_load_3d(sQ + t * kTileBytes + kb * kBlockBytes, &tm_q, kb * 64, g.head0, g.row0 + t * p.tile_tokens, q_full);
+        } else if (ok) {
+          mbar_arrive(q_full);  // no keys: the segment only passes through the barriers that count segments
         }
       }
-      __syncwarp();
-    }
-  } else if (warp == 2) {
-    // =============================== V ===============================
-    uint32_t n_seg = 0, n_tile = 0;
-    int ok = 1;
-    while (ok) {
-      const int slot = n_seg % kSegRing;
-      ok = __all_sync(0xffffffffu, mbar_wait(&seg_full[slot], (n_seg / kSegRing) & 1, p.status));
-      if (!ok) break;
-      const ChunkSegment g = segs[slot];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&seg_empty[slot]);
-      if (g.end) break;
-      ++n_seg;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      prev_alternate = alternate != 0;
+      // (the next segment is announced before this one's V tiles, so that its K can be on the way)
+      if (ok) ok = publish();
+      // ---- V ----
+      const int key_lo = g.key_lo, key_hi = g.key_hi, kv_head = g.kv_head;
       const uint32_t* pages = p.page_table + (size_t)g.seq * p.max_pages_per_seq;
-      for (int j = g.kt0; j < g.kt1 && ok; ++j, ++n_tile) {
+      for (int j = kt0; j < kt1 && ok; ++j, ++n_tile) {
         const int st = n_tile % ST;
-        const int pg0 = max(0, g.key_lo - j * kTile) / TPP;
-        const int pg1 = (min(kTile, g.key_hi - j * kTile) + TPP - 1) / TPP;
+        const int pg0 = max(0, key_lo - j * kTile) / TPP, pg1 = (min(kTile, key_hi - j * kTile) + TPP - 1) / TPP;
         uint32_t pid = 0;
         if (lane >= pg0 && lane < pg1) {
           pid = pages[j * kPagesPerTile + lane];
           if ((long long)pid >= p.num_pages) pid = (uint32_t)(p.num_pages - 1);
         }
-        if (lane == 0) {
-          ok = mbar_wait(&v_empty[st], ((n_tile / ST) & 1) ^ 1, p.status);
-          if (ok) mbar_arrive_expect_tx(&v_full[st], (pg1 - pg0) * kPageBytes);
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], ((n_tile / ST) & 1) ^ 1, p.status)))) break;
+        if (lane == 0) mbar_arrive_expect_tx(&v_full[st], (pg1 - pg0) * kPageBytes);
+        __syncwarp();
         if (lane >= pg0 && lane < pg1)
-          tma_load_3d(sV + st * kTileBytes + lane * kPageBytes, &tm_vpool, 0, 0, (int)(pid * p.num_kv_heads + g.kv_head), &v_full[st]);
+          tma_load_3d(sV + st * kTileBytes + lane * kPageBytes, &tm_vpool, 0, 0, (int)(pid * p.num_kv_heads + kv_head), &v_full[st]);
       }
     }
+    if (lane == 0 && share0 < share1 && !cut_written) p.cuts[blockIdx.x].parts = 0;
+  } else if (warp == 1 || warp == 2) {
+    // =============================== MMA issuers: QK^T and PV ===============================
+    // A segment is a list of steps, one per (key tile, accumulator).  QK^T of step k goes into the S buffer as soon as the
+    // softmax warps have read the scores before it (into registers: a step's QK^T runs under the softmax of the step
+    // before it), PV of step k when its P is there.  The two share nothing but barriers, so each has a warp: one warp that
+    // issues both spends more time on the issue (8 MMAs, waits and commits: ~600 cycles each) than the MMAs take.
+    constexpr int F = Fmt<T>::kCode;
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)) != 0; };
+    auto commit = [&](uint64_t* bar) {
+      if (elect_one()) tc_commit(bar);
+    };
+    // (broadcast: the issuing code is warp-uniform, which the compiler cannot know of values from shared memory)
+    auto uniform = [&](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const bool is_qk = warp == 1;
+    uint32_t n_seg = 0;
+    uint32_t n_tile = 0;            // key tiles whose last MMA has been issued
+    uint32_t n_a0 = 0, n_a1 = 0;    // steps of each accumulator so far
+    int last_acc = -1;              // whose scores the single S buffer holds
+    bool ok = true;
+    while (ok) {
+      const int slot = n_seg % kSegRing;
+      ok = wait_all(&seg_full[slot], (n_seg / kSegRing) & 1);
+      if (!ok) break;
+      const ChunkSegment& sg = segs[slot];
+      const bool residual = uniform(chunk_feeds_residual<T>(p, sg) ? 1 : 0) != 0;
+      const int end = uniform(sg.end), kt0 = uniform(sg.kt0), num = uniform(sg.kt1) - kt0, key_lo = uniform(sg.key_lo), key_hi = uniform(sg.key_hi);
+      const int pair = NQ == 2 && !uniform(sg.alternate) ? 1 : 0;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[slot]);
+      if (end) break;
+      ++n_seg;
+      const int steps = pair ? 2 * num : num;
+      if (is_qk) {
+        constexpr uint32_t idesc_qk = make_idesc(128, F, F, 0);
+        // An operand's descriptor is its constant upper half and (address >> 4) plus a constant: 32-bit arithmetic per MMA.
+        constexpr uint32_t hi_q = (1024u >> 4) | (1u << 14) | (uint32_t)(kLayoutSw128 << 29);
+        constexpr uint32_t hi_k = (128u >> 4) | (1u << 14) | (uint32_t)(kLayoutNone << 29);
+        const uint32_t lo_q = (smem_u32(sQ) >> 4) | (1u << 16);
+        const uint32_t lo_k = (smem_u32(sK) >> 4) | ((B::kChunkBytes >> 4) << 16);
+        ok = wait_all(q_full, (n_seg - 1) & 1);
+        if (ok && num <= 0 && lane == 0) mbar_arrive(q_empty);
+        for (int k = 0; k < steps && ok; ++k) {
+          const int acc = NQ == 2 ? k & 1 : 0, st = n_tile % ST;
+          // the buffer's previous scores have been read
+          const int user = NS == 2 ? acc : last_acc;
+          const uint32_t uses = user == 1 ? n_a1 : n_a0;
+          if (user >= 0 && uses > 0 && !(ok = wait_all(&s_empty[user], (uses - 1) & 1))) break;
+          if ((!pair || acc == 0) && !(ok = wait_all(&k_full[st], (n_tile / ST) & 1))) break;
+          tc_fence_after();
+          const uint32_t d_tmem = tmem_base + (NS == 2 ? acc * kTile : 0), a = lo_q + (pair ? acc : 0) * (kTileBytes >> 4), b = lo_k + st * (kTileBytes >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+              tc_mma_ss32(d_tmem, a + (((ks >> 2) * kBlockBytes + (ks & 3) * 32) >> 4), hi_q, b + ((ks * 2 * B::kChunkBytes) >> 4), hi_k, idesc_qk, ks > 0);
+            tc_commit(&s_full[acc]);
+            if (!pair || acc == 1) tc_commit(&k_empty[st]);
+            if (k == steps - 1) tc_commit(q_empty);
+          }
+          __syncwarp();
+          if (acc) ++n_a1; else ++n_a0;
+          last_acc = acc;
+          if (!pair || acc == 1) ++n_tile;
+        }
+      } else {
+        constexpr uint32_t idesc_pv = make_idesc(D, F, F, 0);
+        constexpr uint32_t hi_v = ((8u * TPP * 2) >> 4) | (1u << 14) | (uint32_t)((TPP == 16 ? kLayoutSw32 : kLayoutSw64) << 29);
+        const uint32_t lo_v = (smem_u32(sV) >> 4) | (1u << 16);
+        constexpr auto off = [](int kk) { return (TPP == 16 ? kk * kPageBytes : (kk >> 1) * kPageBytes + (kk & 1) * 32) >> 4; };
+        for (int k = 0; k < steps && ok; ++k) {
+          const int acc = NQ == 2 ? k & 1 : 0, st = n_tile % ST, i = pair ? k >> 1 : k, j = kt0 + i;
+          const int kk0 = max(0, key_lo - j * kTile) >> 4, kk1 = (min(kTile, key_hi - j * kTile) + 15) >> 4;  // 16-key steps in use
+          const uint32_t fresh = (pair ? i == 0 : k < NQ) ? 1 : 0;                                            // the accumulator starts here
+          if ((!pair || acc == 0) && !(ok = wait_all(&v_full[st], (n_tile / ST) & 1))) break;
+          if (!(ok = wait_all(&p_full[acc], (acc ? n_a1 : n_a0) & 1))) break;
+          tc_fence_after();
+          const uint32_t d_tmem = tmem_base + C::kOCol + acc * B::DP, a = tmem_base + C::kPCol + acc * 64, b = lo_v + st * (kTileBytes >> 4);
+          if (elect_one()) {
+            if (kk0 == 0 && kk1 == kTile / 16) {
+              tc_mma_ts32(d_tmem, a, b, hi_v, idesc_pv, !fresh);
+#pragma unroll
+              for (int kk = 1; kk < kTile / 16; ++kk) tc_mma_ts32(d_tmem, a + kk * 8, b + off(kk), hi_v, idesc_pv, 1);
+            } else {
+#pragma unroll 1
+              for (int kk = kk0; kk < kk1; ++kk) tc_mma_ts32(d_tmem, a + kk * 8, b + off(kk), hi_v, idesc_pv, !(fresh && kk == kk0));
+            }
+            if (residual) {
+              const uint32_t r = tmem_base + (NS == 2 ? acc * kTile : 0);
+#pragma unroll 1
+              for (int kk = kk0; kk < kk1; ++kk) tc_mma_ts32(d_tmem, r + kk * 8, b + off(kk), hi_v, idesc_pv, 1);
+            }
+            tc_commit(&o_done[acc]);
+            if (!pair || acc == 1) tc_commit(&v_empty[st]);
+          }
+          __syncwarp();
+          if (acc) ++n_a1; else ++n_a0;
+          if (!pair || acc == 1) ++n_tile;
+        }
+      }
+    }
+  } else {
+    // =============================== K ===============================
+    // K comes by 16-byte asynchronous copies, lane = token: a page keeps the tokens of a chunk in a row, so 32 lanes write 512
+    // contiguous bytes and read two page rows.  (A TMA gather of four page rows per request brings the same tile in 2590
+    // cycles, these copies in less than 1200, the turn-around of the ring it was measured with.)
+    uint32_t n_seg = 0, n_tile = 0;
+    int pending = -1;  // stage whose K copies have been issued, but not yet been handed over
+    bool ok = true;
+    auto hand_over = [&](auto keep) {  // all copies but the newest `keep` groups have landed
+      if (pending < 0) return;
+      asm volatile("cp.async.wait_group %0;" ::"n"(decltype(keep)::value) : "memory");
+      fence_proxy_async_smem();  // (read by MMAs)
+      mbar_arrive(&k_full[pending]);
+      pending = -1;
+    };
+    // a wait that may last hands over first what may be waited for
+    auto wait_stage = [&](uint64_t* bar, uint32_t parity) {
+      if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+      hand_over(std::integral_constant<int, 0>());
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)) != 0;
+    };
+    while (ok) {
+      const int slot = n_seg % kSegRing;
+      if (!(ok = wait_stage(&seg_full[slot], (n_seg / kSegRing) & 1))) break;
+      const int end = segs[slot].end, kt0 = segs[slot].kt0, kt1 = segs[slot].kt1, key_lo = segs[slot].key_lo, key_hi = segs[slot].key_hi;
+      const int kv_head = segs[slot].kv_head;
+      const uint32_t* pages = p.page_table + (size_t)segs[slot].seq * p.max_pages_per_seq;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[slot]);
+      if (end) {
+        hand_over(std::integral_constant<int, 0>());
+        break;
+      }
+      ++n_seg;
+      // pages [first, last] of key tile j hold visible keys; the others are not touched (their columns of S are masked)
+      auto first_page = [&](int j) { return max(0, key_lo - j * kTile) / TPP; };
+      auto last_page = [&](int j) { return (min(kTile, key_hi - j * kTile) - 1) / TPP; };
+      auto page_id = [&](int j) {  // lane l: the id of page l of the tile (of the nearest one in use)
+        uint32_t pid = 0;
+        if (lane < kPagesPerTile && j < kt1) {
+          pid = pages[j * kPagesPerTile + min(max(lane, first_page(j)), last_page(j))];
+          if ((long long)pid >= p.num_pages) pid = (uint32_t)(p.num_pages - 1);
+        }
+        return pid;
+      };
+      uint32_t next_pid = page_id(kt0);
+      for (int j = kt0; j < kt1; ++j, ++n_tile) {
+        const int st = n_tile % ST;
+        const uint32_t pid = next_pid;
+        next_pid = page_id(j + 1);
+        const int pg0 = first_page(j), pg1 = last_page(j) + 1;
+        if (!(ok = wait_stage(&k_empty[st], ((n_tile / ST) & 1) ^ 1))) break;
+        const uint32_t k_dst = smem_u32(sK) + st * kTileBytes + lane * 16;
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          const int tok = q * 32 + lane, pg = tok / TPP;
+          const uint32_t id = __shfl_sync(0xffffffffu, pid, pg);
+          const unsigned char* src = static_cast<const unsigned char*>(p.k_pool) + ((size_t)id * p.num_kv_heads + kv_head) * kPageBytes + (tok % TPP) * 16;
+          if (pg >= pg0 && pg < pg1)
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(k_dst + q * 512 + c * B::kChunkBytes), "l"(src + c * (TPP * 16)) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        hand_over(std::integral_constant<int, 1>());
+        pending = st;
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   } else {
     if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -690,20 +740,18 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
     const int wg = (warp - 4) >> 2;
     const int lane_group = warp & 3;
     const int row = lane_group * 32 + lane;
+    unsigned char* stage = smem + C::kStage + (warp - 4) * 4096;
     const uint32_t lane_addr = (uint32_t)(lane_group * 32) << 16;
-    const uint32_t tO = tmem_base + lane_addr + B::kOBase + wg * B::DP;
+    const uint32_t tO = tmem_base + lane_addr + C::kOCol + wg * B::DP, tP = tmem_base + lane_addr + C::kPCol + wg * 64;
+    const uint32_t tS = tmem_base + lane_addr + (NS == 2 ? wg * kTile : 0);
     auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)) != 0; };
-    // Phases: with one S buffer the s_full of this accumulator has completed n_s times and its o_done n_o times; with two
-    // buffers, taken in turns, both follow from the number of key tiles n_v.
-    uint32_t n_seg = 0, n_s = 0, n_o = 0, n_v = 0, n_merge = 0;
+    uint32_t n_seg = 0, n_s = 0, n_o = 0, n_v = 0, n_merge = 0;  // segments, scores taken, PVs seen to end, key tiles, merges
     bool ok = true;
     while (ok) {
       const int slot = n_seg % kSegRing;
       ok = wait_all(&seg_full[slot], (n_seg / kSegRing) & 1);
       if (!ok) break;
-      const ChunkSegment g = segs[slot];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&seg_empty[slot]);
+      const ChunkSegment& g = segs[slot];  // (held until the segment is done: what the epilogue needs stays in shared memory)
       if (g.end) break;
       ++n_seg;
       const bool alt = NQ == 2 && g.alternate;
@@ -718,49 +766,70 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       const int pos = g.pos0 + tok_first + tok;
       const int hi = p.causal ? min(pos, g.key_cap - 1) : g.key_cap - 1;
       const int lo = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
-      // ... and the narrowest range over the tile's tokens: key tiles inside it need no mask
-      const int pos_a = g.pos0 + tok_first, pos_b = pos_a + p.tile_tokens - 1;
+      // ... and the keys that all rows of this warp see, [all_lo, all_hi]
+      const int pos_a = g.pos0 + tok_first + lane_group * 32 / p.tile_heads, pos_b = g.pos0 + tok_first + (lane_group * 32 + 31) / p.tile_heads;
       const int all_hi = p.causal ? min(pos_a, g.key_cap - 1) : g.key_cap - 1;
       const int all_lo = p.window > 0 && pos_b >= p.window ? pos_b - p.window + 1 : 0;
       const bool residual = chunk_feeds_residual<T>(p, g);
       float m_used = -INFINITY, l_run = 0.f;
-      const int num = g.kt1 - g.kt0;
+      const int kt0 = g.kt0, num = g.kt1 - kt0;
       int mine = 0;  // key tiles this accumulator has taken
       for (int i = 0; i < num; ++i) {
         if (alt && (i & 1) != wg) {
           ++n_v;
           continue;
         }
-        const int j = g.kt0 + i;
-        const int si = SBUF == 2 ? (int)(n_v & 1) : wg;
-        const uint32_t tS = tmem_base + lane_addr + si * kTile;
-        if (!(ok = wait_all(&s_full[si], (SBUF == 2 ? n_v >> 1 : n_s) & 1))) break;
+        const int j = kt0 + i;
+        if (!(ok = wait_all(&s_full[wg], n_s & 1))) break;
         ++n_s;
         tc_fence_after();
-        if (warp_works) {
-          uint32_t sc[128];
-          tmem_ld128(tS, sc);
-          tmem_wait_ld();
-          const bool need_mask = (j + 1) * kTile - 1 > all_hi || j * kTile < all_lo;
-          if (need_mask) {
-            const int rh = hi - j * kTile, rl = lo - j * kTile;
-#pragma unroll
-            for (int c = 0; c < 128; ++c)
-              if (c > rh || c < rl) sc[c] = 0xff800000u;
+        auto scores_read = [&]() {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_empty[wg]);
+        };
+        // O and the P tile are this warp's again once the PV of the previous key tile has run
+        bool pv_done = mine == 0 || residual;
+        auto wait_pv = [&]() {
+          if (!pv_done) {
+            if (!wait_all(&o_done[wg], n_o & 1)) return false;
+            ++n_o;
+            tc_fence_after();
+            pv_done = true;
           }
-          const float mx = row_max128(sc) * p.scale_log2;  // scale > 0: the maximum commutes with the scaling
+          return true;
+        };
+        // V rows of slots that no row of the item sees (past the last key, before the window, never written) would be
+        // multiplied by P = 0, which is not 0 if they hold an infinity or a NaN: zero them in the 16-key steps that are used.
+        auto clear_values = [&]() {
+          const int c_lo = max(0, g.key_lo - j * kTile), c_hi = min(kTile, g.key_hi - j * kTile);
+          if (!((c_lo | c_hi) & 15)) return true;
+          const int st = (int)(n_v % ST);
+          if (!wait_all(&v_full[st], (n_v / ST) & 1)) return false;
+          unsigned char* vt = sV + st * kTileBytes;
+          for (int dr = row; dr < D; dr += 128) {
+            const int sw = TPP == 16 ? ((dr >> 2) & 1) : ((dr >> 1) & 3);
+            auto clear = [&](int from, int to) {
+              for (int c = from; c < to; ++c) {
+                const int s = c % TPP;
+                *reinterpret_cast<uint16_t*>(vt + (c / TPP) * kPageBytes + dr * (TPP * 2) + ((((s >> 3) ^ sw) << 4) | ((s & 7) << 1))) = 0;
+              }
+            };
+            clear(c_lo & ~15, c_lo);
+            clear(c_hi, (c_hi + 15) & ~15);
+          }
+          fence_proxy_async_smem();
+          return true;
+        };
+        // takes the row maximum of this tile in; the caller has scaled it (scale > 0: the maximum commutes with the scaling)
+        auto new_max = [&](float mx) {
           const float m_new = fmaxf(m_used, mx);
           if (mine == 0) {
             m_used = m_new;
           } else if (__any_sync(0xffffffffu, m_new > m_used + kRescaleThreshold)) {
-            // O must be stable.  With one S buffer per accumulator QK^T of this tile was issued after PV of the previous
-            // one, so it is; with two, that PV may still run.
-            if (SBUF == 2) {
-              if (!(ok = wait_all(&o_done[(n_v - 1) & 1], ((n_v - 1) >> 1) & 1))) break;
-              tc_fence_after();
-            }
+            if (!wait_pv()) return false;
             const float f = m_new > m_used ? fast_exp2(m_used - m_new) : 1.f;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / kOC; ++c) {
               uint32_t v[kOC];
               tmem_ldw(tO + c * kOC, v);
@@ -772,51 +841,71 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
             l_run *= f;
             m_used = m_new;
           }
+          return true;
+        };
+        // One tile without residual: the row in registers, straight through.  (The masked form is a copy of its own: a branch
+        // around the masking alone makes the compiler spill the scores, at twice the time of every tile.)
+        auto plain_tile = [&](auto masked, int rl, int rh) {
+          uint32_t sc[128];
+          tmem_ld128(tS, sc);
+          tmem_wait_ld();
+          scores_read();
+          if (decltype(masked)::value) {
+#pragma unroll
+            for (int c = 0; c < 128; ++c)
+              if (c < rl || c > rh) sc[c] = 0xff800000u;
+          }
+          if (!new_max(row_max128(sc) * p.scale_log2)) return false;
           const float m_ref = m_used > -INFINITY ? m_used : 0.f;
-          chunk_exp_store<T>(tS, sc, p.scale_log2, m_ref, residual, l_run);
+          float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          uint32_t w[32];
+          chunk_exp_half<T>(sc, 0, p.scale_log2, m_ref, w, acc);
+          if (!wait_pv()) return false;
+          tmem_st32(tP, w);
+          chunk_exp_half<T>(sc, 1, p.scale_log2, m_ref, w, acc);
+          tmem_st32(tP + 32, w);
+          l_run += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
           tmem_wait_st();
+          return true;
+        };
+        if (!warp_works) {
+          if (!residual) scores_read();
+          if (!(ok = wait_pv())) break;
+        } else if (residual) {
+          const int rl = lo - j * kTile, rh = hi - j * kTile;
+          if (!(ok = new_max(chunk_residual_max(tS, rl, rh) * p.scale_log2) && wait_pv())) break;
+          l_run += chunk_residual_exp<T>(tS, tP, rl, rh, p.scale_log2, m_used > -INFINITY ? m_used : 0.f);
+          tmem_wait_st();  // (the score buffer now holds the residual, and is given back after the PV)
+        } else {
+          const int c0 = j * kTile;
+          if (c0 < all_lo || c0 + kTile - 1 > all_hi)
+            ok = plain_tile(std::true_type(), lo - c0, hi - c0);
+          else
+            ok = plain_tile(std::false_type(), 0, 0);
+          if (!ok) break;
         }
         ++mine;
-        // V rows of slots that no row of the item sees (past the last key, before the window, never written) would be
-        // multiplied by P = 0, which is not 0 if they hold an infinity or a NaN: zero them in the 16-key steps that are used.
-        if (wg == 0 || alt) {
-          const int c_lo = max(0, g.key_lo - j * kTile), c_hi = min(kTile, g.key_hi - j * kTile);
-          if ((c_lo | c_hi) & 15) {
-            const int st = (int)(n_v % ST);
-            if (!(ok = wait_all(&v_full[st], (n_v / ST) & 1))) break;
-            unsigned char* vt = sV + st * kTileBytes;
-            for (int dr = row; dr < D; dr += 128) {
-              const int sw = TPP == 16 ? ((dr >> 2) & 1) : ((dr >> 1) & 3);
-              auto clear = [&](int from, int to) {
-                for (int c = from; c < to; ++c) {
-                  const int s = c % TPP;
-                  *reinterpret_cast<uint16_t*>(vt + (c / TPP) * kPageBytes + dr * (TPP * 2) + ((((s >> 3) ^ sw) << 4) | ((s & 7) << 1))) = 0;
-                }
-              };
-              clear(c_lo & ~15, c_lo);
-              clear(c_hi, (c_hi + 15) & ~15);
-            }
-            fence_proxy_async_smem();
-          }
-        }
+        if ((wg == 0 || alt) && !(ok = clear_values())) break;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[si]);
+        if (lane == 0) mbar_arrive(&p_full[wg]);
+        if (residual) {
+          // (the S buffer holds the residual until the PV has run)
+          if (!(ok = wait_all(&o_done[wg], n_o & 1))) break;
+          ++n_o;
+          scores_read();
+        }
         ++n_v;
       }
       if (!ok) break;
       // ---- epilogue ----
-      // O is complete (its last PV committed): NQ = 2 commits once per segment and accumulator that had key tiles
-      if (mine > 0) {
-        if (SBUF == 2) {
-          ok = wait_all(&o_done[(n_v - 1) & 1], ((n_v - 1) >> 1) & 1);
-        } else {
-          ok = wait_all(&o_done[wg], n_o & 1);
-          ++n_o;
-        }
+      // O is complete once the last PV has run
+      if (mine > 0 && !residual) {
+        ok = wait_all(&o_done[wg], n_o & 1);
+        ++n_o;
         if (!ok) break;
-        tc_fence_after();
       }
+      tc_fence_after();
       const bool any = mine > 0 && m_used > -INFINITY;
       float m_row = any ? m_used : -INFINITY, l_row = any ? l_run : 0.f;
       float w_own = any ? 1.f : 0.f, w_other = 0.f;
@@ -833,7 +922,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           ++n_merge;
           if (row / C::kMergeRows == pass && lane_group * 32 < used_rows) {
             sMl[row] = make_float2(m_row, l_row);
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / kOC; ++c) {
               uint32_t v[kOC];
               tmem_ldw(tO + c * kOC, v);
@@ -849,8 +938,6 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
         }
         if (!ok) break;
       } else if (!(alt && wg == 1)) {
-        const long long tok_row = (long long)g.row0 + tok_first + tok;
-        const size_t out_row = (size_t)tok_row * p.num_q_heads + g.head0 + head;
         const int item_row = (tok_first + tok) * p.tile_heads + head;  // row of the item: all accumulator tiles
         for (int pass = 0; pass == 0 || (merge && pass * C::kMergeRows < used_rows); ++pass) {
           if (merge) {
@@ -867,47 +954,42 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
               m_row = m;
             }
             const bool direct = g.slot < 0;
-            const float inv = direct ? (l_row > 0.f ? 1.f / l_row : (l_row == 0.f ? 0.f : l_row)) : 1.f;
+            const float inv = direct ? chunk_inverse_sum(l_row) : 1.f;
             const float f0 = w_own * inv, f1 = w_other * inv;
             if (!direct && row_exists) reinterpret_cast<float2*>(p.part_ml)[(size_t)g.slot * p.part_rows + item_row] = make_float2(m_row, l_row);
+            // columns c * OC .. of this row, scaled and merged
+            auto columns = [&](int c, auto& x) {
+              constexpr int OC = sizeof(x) / sizeof(float);
+              uint32_t v[OC / kOC][kOC];
 #pragma unroll
-            for (int c = 0; c < D / kOC; ++c) {
-              float x[kOC];
-              if (mine > 0) {
-                uint32_t v[kOC];
-                tmem_ldw(tO + c * kOC, v);
-                tmem_wait_ld();
+              for (int h = 0; h < OC / kOC; ++h) tmem_ldw(tO + c * OC + h * kOC, v[h]);
+              tmem_wait_ld();
+              // (a row whose O counts for nothing may hold anything: no key seen, or no PV run at all)
 #pragma unroll
-                for (int k = 0; k < kOC; ++k) x[k] = f0 != 0.f ? __uint_as_float(v[k]) * f0 : 0.f;
-              } else {
-#pragma unroll
-                for (int k = 0; k < kOC; ++k) x[k] = 0.f;
-              }
+              for (int k = 0; k < OC; ++k) x[k] = f0 != 0.f ? __uint_as_float(v[k / kOC][k % kOC]) * f0 : 0.f;
               if (merge && f1 != 0.f) {
 #pragma unroll
-                for (int k = 0; k < kOC / 4; ++k) {
-                  const float4 y = *merge_chunk(c * (kOC / 4) + k);
+                for (int k = 0; k < OC / 4; ++k) {
+                  const float4 y = *merge_chunk(c * (OC / 4) + k);
                   x[4 * k] = fmaf(y.x, f1, x[4 * k]);
                   x[4 * k + 1] = fmaf(y.y, f1, x[4 * k + 1]);
                   x[4 * k + 2] = fmaf(y.z, f1, x[4 * k + 2]);
                   x[4 * k + 3] = fmaf(y.w, f1, x[4 * k + 3]);
                 }
               }
-              if (!row_exists) continue;
-              if (!direct || p.out_f32) {
-                float4* dst = reinterpret_cast<float4*>(direct ? static_cast<float*>(p.out) + out_row * D
-                                                               : p.part_acc + ((size_t)g.slot * p.part_rows + item_row) * D) +
-                              c * (kOC / 4);
-#pragma unroll
-                for (int k = 0; k < kOC / 4; ++k) dst[k] = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
-              } else {
-                uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row * D) + c * (kOC / 8);
-#pragma unroll
-                for (int k = 0; k < kOC / 8; ++k)
-                  dst[k] = make_uint4(Mma16816<T>::pack(x[8 * k], x[8 * k + 1]), Mma16816<T>::pack(x[8 * k + 2], x[8 * k + 3]),
-                                      Mma16816<T>::pack(x[8 * k + 4], x[8 * k + 5]), Mma16816<T>::pack(x[8 * k + 6], x[8 * k + 7]));
-              }
-            }
+            };
+            // (row numbers count from the item's first output row, or from the slot's first)
+            const int to = !row_exists ? -1 : direct ? (tok_first + tok) * p.num_q_heads + head : item_row;
+            const size_t first = direct ? (size_t)g.row0 * p.num_q_heads + g.head0 : (size_t)g.slot * p.part_rows;
+            if (!direct || p.out_f32)
+              chunk_store_rows<D, kOC, 4>(stage, lane, reinterpret_cast<unsigned char*>((direct ? static_cast<float*>(p.out) : p.part_acc) + first * D), to,
+                                          columns, [](const float* x) { return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])); });
+            else
+              chunk_store_rows<D, D % 64 == 0 ? 64 : kOC, 2>(stage, lane, reinterpret_cast<unsigned char*>(static_cast<T*>(p.out) + first * D), to,
+                                                             columns, [](const float* x) {
+                                                               return make_uint4(Mma16816<T>::pack(x[0], x[1]), Mma16816<T>::pack(x[2], x[3]),
+                                                                                 Mma16816<T>::pack(x[4], x[5]), Mma16816<T>::pack(x[6], x[7]));
+                                                             });
           }
           if (merge) {
             __syncwarp();
@@ -919,7 +1001,10 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       tc_fence_before();
       if (alt) fence_proxy_async_smem();  // the merge buffer's next user may be a TMA load
       __syncwarp();
-      if (wg == 0 && lane == 0) mbar_arrive(seg_done);
+      if (lane == 0) {
+        mbar_arrive(&seg_empty[slot]);
+        if (wg == 0) mbar_arrive(seg_done);
+      }
     }
   }
 
@@ -933,7 +1018,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
 
 // ---- host side -------------------------------------------------------------------------------
 template <typename T, int D, int TPP>
-int launch_chunk_typed(const ChunkArgs& a, const ChunkParams& p, int grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+int launch_chunk_typed(const ChunkArgs& a, const ChunkParams& p, int grid, const CUtensorMap& q, const CUtensorMap& v,
                        cudaStream_t stream) {
   constexpr int NQ = chunk_accumulators(D);
   using C = ChunkCfg<D, TPP, NQ>;
@@ -942,13 +1027,14 @@ int launch_chunk_typed(const ChunkArgs& a, const ChunkParams& p, int grid, const
   static DeviceOnce configured;  // one per instantiation
   const int rc = configured.run([&] { return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kTotal); });
   if (rc != 0) return rc;
-  kern<<<grid, C::kThreads, C::kTotal, stream>>>(p, q, k, v);
+  kern<<<grid, C::kThreads, C::kTotal, stream>>>(p, q, v);
   return (int)cudaGetLastError();
 }
 
 template <int D, int TPP>
 int launch_chunk_shape(const ChunkArgs& a, cudaStream_t stream) {
   ChunkParams p;
+  p.k_pool = a.k_pool;
   p.page_table = a.page_table;
   p.seq_lens = a.seq_lens;
   p.cu_seqlens = a.cu_seqlens;
@@ -975,7 +1061,7 @@ int launch_chunk_shape(const ChunkArgs& a, cudaStream_t stream) {
   p.part_ml = reinterpret_cast<float*>(static_cast<unsigned char*>(a.scratch) + plan.ml_offset);
   p.part_acc = reinterpret_cast<float*>(static_cast<unsigned char*>(a.scratch) + plan.acc_offset);
 
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mv;
   {
     const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)a.num_q_heads, (cuuint64_t)a.total_tokens};
     const cuuint64_t strides[2] = {(cuuint64_t)a.q_head_stride * 2, (cuuint64_t)a.q_token_stride * 2};
@@ -988,15 +1074,11 @@ int launch_chunk_shape(const ChunkArgs& a, cudaStream_t stream) {
     const cuuint32_t vbox[3] = {(cuuint32_t)TPP, (cuuint32_t)D, 1};
     if (!encode_map(&mv, a.dtype, 3, a.v_pool, vdims, vstrides, vbox, TPP == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B))
       return -3;
-    const cuuint64_t kdims[2] = {(cuuint64_t)TPP * 8, (cuuint64_t)a.num_pages * a.num_kv_heads * (D / 8)};
-    const cuuint64_t kstrides[1] = {(cuuint64_t)TPP * 16};
-    const cuuint32_t kbox[2] = {(cuuint32_t)TPP * 8, 1};
-    if (!encode_map(&mk, a.dtype, 2, a.k_pool, kdims, kstrides, kbox, CU_TENSOR_MAP_SWIZZLE_NONE)) return -3;
   } else {
-    mk = mv = mq;  // never dereferenced: without pages no row sees a key
+    mv = mq;  // never dereferenced: without pages no row sees a key
   }
-  const int rc = a.dtype == 0 ? launch_chunk_typed<__half, D, TPP>(a, p, plan.grid, mq, mk, mv, stream)
-                              : launch_chunk_typed<__nv_bfloat16, D, TPP>(a, p, plan.grid, mq, mk, mv, stream);
+  const int rc = a.dtype == 0 ? launch_chunk_typed<__half, D, TPP>(a, p, plan.grid, mq, mv, stream)
+                              : launch_chunk_typed<__nv_bfloat16, D, TPP>(a, p, plan.grid, mq, mv, stream);
   if (rc != 0) return rc;
   return launch_chunk_merge(a, plan, p.cuts, p.part_ml, p.part_acc, stream);
 }
