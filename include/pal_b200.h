@@ -150,7 +150,8 @@ typedef struct pal_rows {
   int64_t head_stride;
 } pal_rows;
 
-/* out[t, h, :] = rotation of x[t, h, :].  out may be x (same strides); otherwise the two must not overlap. */
+/* out[t, h, :] = rotation of x[t, h, :].  out may be x (same strides); otherwise the two must not overlap.  head_dim is at
+ * most 8192. */
 int pal_rotary_embedding(const pal_rows* x, const pal_rows* out, const pal_rotation* rotation, int64_t num_tokens,
                          int num_heads, int head_dim, int dtype, void* stream);
 

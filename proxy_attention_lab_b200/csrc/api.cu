@@ -267,6 +267,10 @@ int pal_rotary_embedding(const pal_rows* x, const pal_rows* out, const pal_rotat
     set_error("%s: token and head counts must not be negative, head_dim must be positive", what);
     return PAL_ERR_BAD_ARG;
   }
+  if (head_dim > 8192) {
+    set_error("%s: head_dim (%d) is limited to 8192", what, head_dim);
+    return PAL_ERR_UNSUPPORTED;
+  }
   RotaryArgs a{};
   if (!rotation_args(what, rotation, num_tokens, head_dim, &a.rot)) return PAL_ERR_BAD_ARG;
   if (num_tokens == 0 || num_heads == 0) return PAL_OK;

@@ -9,14 +9,14 @@
 // positions below 2^29); the fraction, at most half a turn, is then good to 2^-25 turns in fp32 and sincospif does the rest.
 //
 // Bound: memory.  A rotated element costs 4 bytes of traffic and ~3 flops; the angle, ~60 instructions, is shared by all
-// heads of a token.  So a thread owns one unit - 2 V elements of a head row, V frequencies - of one token, computes its V
-// sines and cosines once into registers and walks over heads with 16-byte loads and stores (V = 8).  How many heads a thread
-// takes is chosen so that the grid fills the GPU first (a few tokens: one head per thread) and shares angles second.
+// heads of a token.  So a block takes a few tokens, computes their sines and cosines once into shared memory, and then a
+// thread owns one unit - 2 V elements of a head row, V frequencies - of one token, takes its angles into registers and walks
+// over the heads with 16-byte loads and stores (V = 8).  Few tokens: one per block, and the heads spread over all threads;
+// many: eight per block.
 //
-// fill_kv_pages_rotary is one launch of blocks in three roles: rotate the queries into their output, rotate the keys into
-// the K pool, move the values into the V pool.
-//   K pool [P, Hkv, D/8, TPP, 8]: a unit is whole 16-byte chunks; eight lanes take eight consecutive tokens, so that a warp
-//     writes runs of 128 contiguous bytes per chunk while it reads 64 bytes of each token row.
+// fill_kv_pages_rotary is one launch of blocks in two roles: rotate queries and keys, and move the values into the V pool.
+//   K pool [P, Hkv, D/8, TPP, 8]: a unit is whole 16-byte chunks; a warp reads 128 contiguous bytes of a row and writes runs
+//     of a few tokens' neighbouring 16-byte chunks.
 //   V pool [P, Hkv, D, TPP]: eight consecutive slots of a page are 16 contiguous bytes of a head-dim row.  A block stages 64
 //     tokens (and the 7 that follow them) of one head in shared memory and finds the octets: runs of eight tokens that fill
 //     an aligned group of eight slots.  An octet belongs to the block that holds its first token, hence the halo: prompts
@@ -33,7 +33,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kTokensPerTile = 64;               // list tokens a V block owns
 constexpr int kTileTokens = kTokensPerTile + 7;  // ... and stages: the octet that starts at its last token ends 7 later
-constexpr int kKeyLanes = 8;                     // consecutive tokens on consecutive lanes in the K role
+constexpr int kTokensPerBlock = 8;               // of a rotating block, when there are enough tokens to fill the GPU
 
 struct RotaryParams {
   RotationArgs rot;
@@ -42,8 +42,9 @@ struct RotaryParams {
   long long q_out_token_stride, q_out_head_stride;
   FillArgs fill;
   int hq;               // query heads to rotate (0 = none)
-  int q_step, k_step;   // threads that share a (token, unit): thread j takes heads j, j + step, ...
-  unsigned q_blocks, k_blocks, v_blocks;
+  int block_tokens;     // tokens of a rotating block
+  int head_splits;      // rotating blocks that share a group of tokens: each takes a range of heads
+  unsigned v_blocks;
   int v_vec;            // new_values can be read in 16-byte vectors
 };
 
@@ -76,28 +77,20 @@ __device__ __forceinline__ int axis_of(const RotationArgs& r, int i) {
   return i / r.num_axes < r.sections[a] ? a : 0;
 }
 
+// Cosine and sine, times the magnitude, of frequency i at a token's position.
+__device__ __forceinline__ float2 cos_sin(const RotationArgs& r, long long token, int i) {
+  const long long at = axis_of(r, i) * r.positions_axis_stride + token;
+  const double pos = r.positions_64bit ? (double)static_cast<const long long*>(r.positions)[at] : (double)static_cast<const int*>(r.positions)[at];
+  double turns = pos * (double)r.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
+  turns -= rint(turns);
+  float sn, cs;
+  sincospif(2.0f * (float)turns, &sn, &cs);
+  return make_float2(cs * r.magnitude, sn * r.magnitude);
+}
+
 template <int V>
 struct Angles {
   float c[V], s[V];
-  __device__ __forceinline__ void compute(const RotationArgs& r, long long token, int i0) {
-    int axis = -1;
-    double pos = 0.0;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int a = axis_of(r, i0 + e);
-      if (a != axis) {
-        axis = a;
-        const long long at = a * r.positions_axis_stride + token;
-        pos = r.positions_64bit ? (double)static_cast<const long long*>(r.positions)[at] : (double)static_cast<const int*>(r.positions)[at];
-      }
-      double turns = pos * (double)r.inv_freq[i0 + e] * 0.15915494309189533577;  // 1 / (2 pi)
-      turns -= rint(turns);
-      float sn, cs;
-      sincospif(2.0f * (float)turns, &sn, &cs);
-      c[e] = cs * r.magnitude;
-      s[e] = sn * r.magnitude;
-    }
-  }
 };
 
 // Unit u of a head row: two vectors of V elements at `first` and `second`; units past the rotated elements pass through
@@ -168,83 +161,84 @@ __device__ __forceinline__ void destination(const FillArgs& f, long long t, long
   }
 }
 
-// Heads j, j + step, ... of one (token, unit), four at a time so that eight loads are in flight before the first use.
-template <typename T, int V, bool ADJACENT, typename Store>
-__device__ __forceinline__ void walk_heads(const T* row, long long head_stride, int heads, int j, int step, const Unit<V, ADJACENT>& u,
-                                           const Angles<V>& g, Store&& store) {
+// A rotating block: tokens [t0, t0 + block_tokens) of heads [head0, head1), counting the queries' heads first and then the
+// keys'.  `table`: [token][2][num_freqs] cosines and sines.
+template <typename T, int V, bool ADJACENT>
+__device__ __forceinline__ void rotate(const RotaryParams& p, unsigned block, float* table) {
   using W = typename Vec<V>::type;
-  constexpr int kBatch = 4;
-  for (int h0 = j; h0 < heads; h0 += kBatch * step) {
-    Elems<T, V> a[kBatch], b[kBatch];
+  const FillArgs& f = p.fill;
+  const int half = p.rot.num_freqs, head_dim = f.head_dim, tpp = f.tokens_per_page;
+  const int heads = p.hq + (p.src_k.data ? f.num_kv_heads : 0);
+  const int split = (int)(block % (unsigned)p.head_splits);
+  const long long t0 = (long long)(block / (unsigned)p.head_splits) * p.block_tokens;
+  const int tokens = (int)min((long long)p.block_tokens, f.num_tokens - t0);
+  const int per_split = (heads + p.head_splits - 1) / p.head_splits;
+  const int head0 = split * per_split, head1 = min(heads, head0 + per_split);
+  if (head0 >= head1) return;
+  for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
+    const int t = i / half, k = i - t * half;
+    const float2 cs = cos_sin(p.rot, t0 + t, k);
+    table[2 * t * half + k] = cs.x;
+    table[(2 * t + 1) * half + k] = cs.y;
+  }
+  __syncthreads();
+
+  // thread: unit and token of its pair, and every step-th head from its own
+  const int units = (head_dim + 2 * V - 1) / (2 * V), pairs = units * tokens;
+  const int step = pairs < kThreads ? kThreads / pairs : 1;
+  for (int i = threadIdx.x; i < pairs * step; i += kThreads) {
+    const int j = i / pairs, pair = i - j * pairs;
+    const int tl = pair / units, ui = pair - tl * units;
+    const long long t = t0 + tl;
+    const Unit<V, ADJACENT> u(ui, half, head_dim);
+    Angles<V> g;
+    if (u.turns) {
+      const float *c = table + 2 * tl * half + V * ui, *sn = c + half;
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int h = h0 + k * step;
-      if (h >= heads) break;
-      const T* p = row + h * head_stride;
-      a[k].v = *reinterpret_cast<const W*>(p + u.first);
-      if (u.second >= 0) b[k].v = *reinterpret_cast<const W*>(p + u.second);
+      for (int e = 0; e < V; ++e) {
+        g.c[e] = c[e];
+        g.s[e] = sn[e];
+      }
     }
+    const T* q_row = static_cast<const T*>(p.src_q.data) + t * p.src_q.token_stride;
+    const T* k_row = static_cast<const T*>(p.src_k.data) + t * p.src_k.token_stride;
+    T* q_out = static_cast<T*>(p.q_out) + t * p.q_out_token_stride;
+    // element e of a key lies in chunk e / 8 of its (page, head) block, at [chunk][slot][e % 8]
+    long long page = -1;
+    int slot = 0;
+    if (head1 > p.hq) destination(f, t, page, slot);
+    T* pool = static_cast<T*>(f.k_pool) + page * f.num_kv_heads * head_dim * tpp;
+    const int o1 = ((u.first >> 3) * tpp + slot) * 8 + (u.first & 7);
+    const int o2 = u.second >= 0 ? ((u.second >> 3) * tpp + slot) * 8 + (u.second & 7) : 0;
+    // four heads at a time: eight loads are in flight before the first use
+    constexpr int kBatch = 4;
+    for (int h0 = head0 + j; h0 < head1; h0 += kBatch * step) {
+      Elems<T, V> a[kBatch], b[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int h = h0 + k * step;
-      if (h >= heads) break;
-      if (u.turns) turn<T, V, ADJACENT>(a[k], b[k], g);
-      store(h, a[k], b[k]);
+      for (int k = 0; k < kBatch; ++k) {
+        const int h = h0 + k * step;
+        if (h >= head1) break;
+        const T* src = h < p.hq ? q_row + h * p.src_q.head_stride : k_row + (h - p.hq) * p.src_k.head_stride;
+        a[k].v = *reinterpret_cast<const W*>(src + u.first);
+        if (u.second >= 0) b[k].v = *reinterpret_cast<const W*>(src + u.second);
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int h = h0 + k * step;
+        if (h >= head1) break;
+        if (u.turns) turn<T, V, ADJACENT>(a[k], b[k], g);
+        if (h < p.hq) {
+          T* o = q_out + h * p.q_out_head_stride;
+          *reinterpret_cast<W*>(o + u.first) = a[k].v;
+          if (u.second >= 0) *reinterpret_cast<W*>(o + u.second) = b[k].v;
+        } else if (page >= 0) {
+          T* o = pool + (long long)(h - p.hq) * head_dim * tpp;
+          *reinterpret_cast<W*>(o + o1) = a[k].v;
+          if (u.second >= 0) *reinterpret_cast<W*>(o + o2) = b[k].v;
+        }
+      }
     }
   }
-}
-
-template <typename T, int V, bool ADJACENT>
-__device__ __forceinline__ void rotate_queries(const RotaryParams& p, long long tid, int units) {
-  const int head_dim = p.fill.head_dim, half = p.rot.num_freqs;
-  const int ui = (int)(tid % units);
-  const long long r = tid / units;
-  const int j = (int)(r % p.q_step);
-  const long long t = r / p.q_step;
-  if (t >= p.fill.num_tokens) return;
-  const Unit<V, ADJACENT> u(ui, half, head_dim);
-  Angles<V> g;
-  if (u.turns) g.compute(p.rot, t, V * ui);
-  using W = typename Vec<V>::type;
-  T* out = static_cast<T*>(p.q_out) + t * p.q_out_token_stride;
-  walk_heads<T, V, ADJACENT>(static_cast<const T*>(p.src_q.data) + t * p.src_q.token_stride, p.src_q.head_stride, p.hq, j, p.q_step, u, g,
-                             [&](int h, const Elems<T, V>& a, const Elems<T, V>& b) {
-                               T* o = out + h * p.q_out_head_stride;
-                               *reinterpret_cast<W*>(o + u.first) = a.v;
-                               if (u.second >= 0) *reinterpret_cast<W*>(o + u.second) = b.v;
-                             });
-}
-
-template <typename T, int V, bool ADJACENT>
-__device__ __forceinline__ void rotate_keys(const RotaryParams& p, long long tid, int units) {
-  const FillArgs& f = p.fill;
-  const int half = p.rot.num_freqs;
-  const int tl = (int)(tid % kKeyLanes);
-  long long r = tid / kKeyLanes;
-  const int ui = (int)(r % units);
-  r /= units;
-  const int j = (int)(r % p.k_step);
-  const long long t = r / p.k_step * kKeyLanes + tl;
-  if (t >= f.num_tokens) return;
-  long long page;
-  int slot;
-  destination(f, t, page, slot);
-  if (page < 0) return;
-  const Unit<V, ADJACENT> u(ui, half, f.head_dim);
-  Angles<V> g;
-  if (u.turns) g.compute(p.rot, t, V * ui);
-  using W = typename Vec<V>::type;
-  const int tpp = f.tokens_per_page;
-  // element e of a head lies in chunk e / 8 at [chunk][slot][e % 8]
-  const long long o1 = ((long long)(u.first >> 3) * tpp + slot) * 8 + (u.first & 7);
-  const long long o2 = u.second >= 0 ? ((long long)(u.second >> 3) * tpp + slot) * 8 + (u.second & 7) : 0;
-  T* pool = static_cast<T*>(f.k_pool) + page * f.num_kv_heads * f.head_dim * tpp;
-  walk_heads<T, V, ADJACENT>(static_cast<const T*>(p.src_k.data) + t * p.src_k.token_stride, p.src_k.head_stride, f.num_kv_heads, j, p.k_step,
-                             u, g, [&](int h, const Elems<T, V>& a, const Elems<T, V>& b) {
-                               T* o = pool + (long long)h * f.head_dim * tpp;
-                               *reinterpret_cast<W*>(o + o1) = a.v;
-                               if (u.second >= 0) *reinterpret_cast<W*>(o + o2) = b.v;
-                             });
 }
 
 __device__ __forceinline__ void copy_async_16(uint32_t smem_dst, const void* src) {
@@ -348,36 +342,19 @@ __device__ __forceinline__ void move_values(const RotaryParams& p, unsigned bloc
 template <typename T, int V, bool ADJACENT>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
   extern __shared__ __align__(128) unsigned char rotary_smem[];
-  const int units = (p.fill.head_dim + 2 * V - 1) / (2 * V);
-  unsigned b = blockIdx.x;
-  if (b < p.v_blocks) {
-    move_values(p, b, rotary_smem);
-    return;
-  }
-  b -= p.v_blocks;
-  if (b < p.k_blocks) {
-    rotate_keys<T, V, ADJACENT>(p, (long long)b * kThreads + threadIdx.x, units);
-    return;
-  }
-  b -= p.k_blocks;
-  rotate_queries<T, V, ADJACENT>(p, (long long)b * kThreads + threadIdx.x, units);
+  if (blockIdx.x < p.v_blocks)
+    move_values(p, blockIdx.x, rotary_smem);
+  else
+    rotate<T, V, ADJACENT>(p, blockIdx.x - p.v_blocks, reinterpret_cast<float*>(rotary_smem));
 }
 
 bool aligned_rows(const void* data, long long token_stride, long long head_stride, int bytes) {
   return reinterpret_cast<uintptr_t>(data) % bytes == 0 && (token_stride * 2) % bytes == 0 && (head_stride * 2) % bytes == 0;
 }
 
-// Threads that share a (token, unit): as many as it takes for every SM to hold 1024 threads, at most one per head.  With
-// more tokens than that a thread takes several heads and the angles are computed once for them.
-int head_step(long long token_units, int heads) {
-  const long long want = 148LL * 1024;
-  long long step = (want + token_units - 1) / token_units;
-  return (int)(step < 1 ? 1 : (step > heads ? heads : step));
-}
-
 template <typename T, int V, bool ADJACENT>
-int launch_inst(const RotaryParams& p, size_t smem, cudaStream_t stream) {
-  const unsigned long long blocks = (unsigned long long)p.q_blocks + p.k_blocks + p.v_blocks;
+int launch_inst(const RotaryParams& p, unsigned long long rotating, size_t smem, cudaStream_t stream) {
+  const unsigned long long blocks = rotating + p.v_blocks;
   if (blocks > 0x7fffffffULL) {
     set_error("rotary: too many tokens for one launch");
     return -2;
@@ -387,11 +364,11 @@ int launch_inst(const RotaryParams& p, size_t smem, cudaStream_t stream) {
 }
 
 template <typename T>
-int launch_typed(const RotaryParams& p, int vec, size_t smem, cudaStream_t stream) {
+int launch_typed(const RotaryParams& p, int vec, unsigned long long rotating, size_t smem, cudaStream_t stream) {
   const bool adjacent = p.rot.pairing == 1;
-  if (vec == 8) return adjacent ? launch_inst<T, 8, true>(p, smem, stream) : launch_inst<T, 8, false>(p, smem, stream);
-  if (vec == 4) return adjacent ? launch_inst<T, 4, true>(p, smem, stream) : launch_inst<T, 4, false>(p, smem, stream);
-  return adjacent ? launch_inst<T, 1, true>(p, smem, stream) : launch_inst<T, 1, false>(p, smem, stream);
+  if (vec == 8) return adjacent ? launch_inst<T, 8, true>(p, rotating, smem, stream) : launch_inst<T, 8, false>(p, rotating, smem, stream);
+  if (vec == 4) return adjacent ? launch_inst<T, 4, true>(p, rotating, smem, stream) : launch_inst<T, 4, false>(p, rotating, smem, stream);
+  return adjacent ? launch_inst<T, 1, true>(p, rotating, smem, stream) : launch_inst<T, 1, false>(p, rotating, smem, stream);
 }
 
 }  // namespace
@@ -422,23 +399,25 @@ int launch_rotary(const RotaryArgs& a, cudaStream_t stream) {
       break;
     }
   }
-  const long long units = (d + 2 * vec - 1) / (2 * vec);
-  size_t smem = 0;
-  auto blocks_for = [](long long threads) { return (unsigned)((threads + kThreads - 1) / kThreads); };
-  if (p.hq > 0) {
-    p.q_step = head_step(tokens * units, p.hq);
-    p.q_blocks = blocks_for(tokens * units * p.q_step);
-  }
+  const int heads = p.hq + (a.k.data ? a.fill.num_kv_heads : 0);
+  // Eight tokens share a block once that gives every SM one; below, a token has blocks of its own, one per as many heads as
+  // its threads hold at once while the GPU has room for them.
+  const long long sms = cached_sm_count();
+  p.block_tokens = tokens >= kTokensPerBlock * sms && half <= 768 ? kTokensPerBlock : 1;  // (their table stays within 48 KB)
+  const long long groups = (tokens + p.block_tokens - 1) / p.block_tokens;
+  const int units = (d + 2 * vec - 1) / (2 * vec);
+  const int at_once = kThreads / units > 1 ? kThreads / units : 1;
+  const long long splits_wanted = (heads + at_once - 1) / at_once, splits_room = 4 * sms / groups;
+  p.head_splits = (int)(splits_room < 1 ? 1 : (splits_room < splits_wanted ? splits_room : splits_wanted));
+  size_t smem = (size_t)p.block_tokens * 2 * half * sizeof(float);
   if (a.k.data) {
-    const long long groups = (tokens + kKeyLanes - 1) / kKeyLanes;
-    p.k_step = head_step(groups * kKeyLanes * units, a.fill.num_kv_heads);
-    p.k_blocks = blocks_for(groups * kKeyLanes * units * p.k_step);
     p.v_blocks = (unsigned)((tokens + kTokensPerTile - 1) / kTokensPerTile * a.fill.num_kv_heads);
     p.v_vec = aligned_rows(a.v.data, a.v.token_stride, a.v.head_stride, 16) ? 1 : 0;
-    const int rows = (int)(tokens < kTileTokens ? tokens : kTileTokens);
-    smem = (size_t)rows * ((d / 8 + 7) / 8 * 128);
+    const size_t rows = (size_t)(tokens < kTileTokens ? tokens : kTileTokens) * ((d / 8 + 7) / 8 * 128);
+    if (rows > smem) smem = rows;
   }
-  return a.dtype == 0 ? launch_typed<__half>(p, vec, smem, stream) : launch_typed<__nv_bfloat16>(p, vec, smem, stream);
+  const unsigned long long rotating = (unsigned long long)groups * p.head_splits;
+  return a.dtype == 0 ? launch_typed<__half>(p, vec, rotating, smem, stream) : launch_typed<__nv_bfloat16>(p, vec, rotating, smem, stream);
 }
 
 }  // namespace pal

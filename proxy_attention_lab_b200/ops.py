@@ -364,6 +364,13 @@ def rotary_embedding(x, positions, inv_freq, *, sections=None, section_order: st
     ``x``, but must not overlap it otherwise).  Negated positions undo the rotation; the gradient of ``x`` is the rotation of
     the output's gradient by the negated positions.
     """
+    if _fast is not None and stream is None and out is None and pairing in ROTARY_PAIRING and section_order in SECTION_ORDER:
+        try:
+            done = _fast.rotary(x, positions, inv_freq, sections, SECTION_ORDER[section_order], ROTARY_PAIRING[pairing], magnitude)
+        except TypeError:
+            done = None
+        if done is not None:
+            return done
     _need_cuda("x", x)
     if x.dim() != 3:
         raise ValueError("x must be 3-D [tokens, heads, head_dim]")
@@ -415,6 +422,16 @@ def fill_kv_pages_rotary(
     """
     if slot_mapping is None and page_table is not None and current_token_write_positions is None and query_to_seq_map is None:
         slot_mapping, page_table = page_table, None
+    if (_fast is not None and stream is None and inplace and queries_out is None and pairing in ROTARY_PAIRING and section_order in SECTION_ORDER
+            and (slot_mapping is None or page_table is None)):
+        try:
+            done = _fast.fill_rotary(new_keys, new_values, global_key_pool, global_value_pool, page_table if slot_mapping is None else slot_mapping,
+                                     current_token_write_positions, query_to_seq_map, positions, inv_freq, sections, SECTION_ORDER[section_order],
+                                     ROTARY_PAIRING[pairing], magnitude, queries)
+        except TypeError:
+            done = None
+        if done is not None:
+            return (global_key_pool, global_value_pool) if queries is None else (global_key_pool, global_value_pool, done)
     for name, t in (("new_keys", new_keys), ("new_values", new_values), ("global_key_pool", global_key_pool),
                     ("global_value_pool", global_value_pool)):
         _need_cuda(name, t)
@@ -869,6 +886,15 @@ def paged_attention_chunk(queries, k_cache_pool, v_cache_pool, page_table, seque
     ``out_dtype=torch.float32``, written to ``out`` if given.  Rows that belong to no sequence (behind ``cu_seqlens[S]``) are
     not written.
     """
+    if _fast is not None and stream is None and (out_dtype is None or out_dtype is torch.float32) and (window is None or (causal and window > 0)):
+        try:
+            done = _fast.chunk(queries, k_cache_pool, v_cache_pool, page_table, sequence_lengths, cu_seqlens, bool(causal),
+                               0 if window is None else int(window), 0.0 if scale is None else float(scale), out_dtype is torch.float32, out,
+                               _STATUS_PAGES)
+        except TypeError:
+            done = None
+        if done is not None:
+            return done
     for name, t in (("queries", queries), ("k_cache_pool", k_cache_pool), ("v_cache_pool", v_cache_pool), ("page_table", page_table),
                     ("sequence_lengths", sequence_lengths)):
         _need_cuda(name, t)
