@@ -12,7 +12,7 @@
 // heads of a token.  So a block takes a few tokens, computes their sines and cosines once into shared memory, and then a
 // thread owns one unit - 2 V elements of a head row, V frequencies - of one token, takes its angles into registers and walks
 // over the heads with 16-byte loads and stores (V = 8).  Few tokens: one per block, and the heads spread over all threads;
-// many: eight per block.
+// many: sixteen per block.
 //
 // fill_kv_pages_rotary is one launch of blocks in two roles: rotate queries and keys, and move the values into the V pool.
 //   K pool [P, Hkv, D/8, TPP, 8]: a unit is whole 16-byte chunks; a warp reads 128 contiguous bytes of a row and writes runs
@@ -31,9 +31,9 @@ namespace pal {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTokensPerTile = 64;               // list tokens a V block owns
+constexpr int kTokensPerTile = 64;               // list tokens a V block owns (8 where that leaves SMs idle)
 constexpr int kTileTokens = kTokensPerTile + 7;  // ... and stages: the octet that starts at its last token ends 7 later
-constexpr int kTokensPerBlock = 8;               // of a rotating block, when there are enough tokens to fill the GPU
+constexpr int kTokensPerBlock = 16;              // of a rotating block, when there are enough tokens to fill the GPU
 
 struct RotaryParams {
   RotationArgs rot;
@@ -45,6 +45,7 @@ struct RotaryParams {
   int block_tokens;     // tokens of a rotating block
   int head_splits;      // rotating blocks that share a group of tokens: each takes a range of heads
   unsigned v_blocks;
+  int v_tokens;         // tokens a V block owns
   int v_vec;            // new_values can be read in 16-byte vectors
 };
 
@@ -175,18 +176,38 @@ __device__ __forceinline__ void rotate(const RotaryParams& p, unsigned block, fl
   const int per_split = (heads + p.head_splits - 1) / p.head_splits;
   const int head0 = split * per_split, head1 = min(heads, head0 + per_split);
   if (head0 >= head1) return;
-  for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
-    const int t = i / half, k = i - t * half;
+  // thread: unit and token of its pair, and every step-th head from its own
+  const int units = (head_dim + 2 * V - 1) / (2 * V), pairs = units * tokens;
+  const int step = pairs < kThreads ? kThreads / pairs : 1;
+  constexpr int kBatch = 2;  // heads at a time (four: 92 -> 100 us for 16384 tokens, the registers cost resident blocks)
+  Elems<T, V> a[kBatch], b[kBatch];
+  auto load = [&](const Unit<V, ADJACENT>& u, long long t, int h0) {
+    const T* q_row = static_cast<const T*>(p.src_q.data) + t * p.src_q.token_stride;
+    const T* k_row = static_cast<const T*>(p.src_k.data) + t * p.src_k.token_stride;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int h = h0 + k * step;
+      if (h >= head1) break;
+      const T* src = h < p.hq ? q_row + h * p.src_q.head_stride : k_row + (h - p.hq) * p.src_k.head_stride;
+      a[k].v = *reinterpret_cast<const W*>(src + u.first);
+      if (u.second >= 0) b[k].v = *reinterpret_cast<const W*>(src + u.second);
+    }
+  };
+  // the first heads travel while the angles are computed
+  int i = threadIdx.x;
+  if (i < pairs * step) {
+    const int j = i / pairs, pair = i - j * pairs, tl = pair / units;
+    load(Unit<V, ADJACENT>(pair - tl * units, half, head_dim), t0 + tl, head0 + j);
+  }
+  for (int e = threadIdx.x; e < tokens * half; e += kThreads) {
+    const int t = e / half, k = e - t * half;
     const float2 cs = cos_sin(p.rot, t0 + t, k);
     table[2 * t * half + k] = cs.x;
     table[(2 * t + 1) * half + k] = cs.y;
   }
   __syncthreads();
 
-  // thread: unit and token of its pair, and every step-th head from its own
-  const int units = (head_dim + 2 * V - 1) / (2 * V), pairs = units * tokens;
-  const int step = pairs < kThreads ? kThreads / pairs : 1;
-  for (int i = threadIdx.x; i < pairs * step; i += kThreads) {
+  for (bool loaded = true; i < pairs * step; i += kThreads) {
     const int j = i / pairs, pair = i - j * pairs;
     const int tl = pair / units, ui = pair - tl * units;
     const long long t = t0 + tl;
@@ -200,8 +221,6 @@ __device__ __forceinline__ void rotate(const RotaryParams& p, unsigned block, fl
         g.s[e] = sn[e];
       }
     }
-    const T* q_row = static_cast<const T*>(p.src_q.data) + t * p.src_q.token_stride;
-    const T* k_row = static_cast<const T*>(p.src_k.data) + t * p.src_k.token_stride;
     T* q_out = static_cast<T*>(p.q_out) + t * p.q_out_token_stride;
     // element e of a key lies in chunk e / 8 of its (page, head) block, at [chunk][slot][e % 8]
     long long page = -1;
@@ -210,18 +229,9 @@ __device__ __forceinline__ void rotate(const RotaryParams& p, unsigned block, fl
     T* pool = static_cast<T*>(f.k_pool) + page * f.num_kv_heads * head_dim * tpp;
     const int o1 = ((u.first >> 3) * tpp + slot) * 8 + (u.first & 7);
     const int o2 = u.second >= 0 ? ((u.second >> 3) * tpp + slot) * 8 + (u.second & 7) : 0;
-    // four heads at a time: eight loads are in flight before the first use
-    constexpr int kBatch = 4;
     for (int h0 = head0 + j; h0 < head1; h0 += kBatch * step) {
-      Elems<T, V> a[kBatch], b[kBatch];
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int h = h0 + k * step;
-        if (h >= head1) break;
-        const T* src = h < p.hq ? q_row + h * p.src_q.head_stride : k_row + (h - p.hq) * p.src_k.head_stride;
-        a[k].v = *reinterpret_cast<const W*>(src + u.first);
-        if (u.second >= 0) b[k].v = *reinterpret_cast<const W*>(src + u.second);
-      }
+      if (!loaded) load(u, t, h0);
+      loaded = false;
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         const int h = h0 + k * step;
@@ -266,9 +276,9 @@ __device__ __forceinline__ void move_values(const RotaryParams& p, unsigned bloc
   __shared__ int s_num_octets, s_num_singles;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int head = (int)(block % (unsigned)f.num_kv_heads);
-  const long long t0 = (long long)(block / (unsigned)f.num_kv_heads) * kTokensPerTile;
-  const int rows = (int)min((long long)kTileTokens, f.num_tokens - t0);
-  const int owned = min(rows, kTokensPerTile);
+  const long long t0 = (long long)(block / (unsigned)f.num_kv_heads) * p.v_tokens;
+  const int rows = (int)min((long long)p.v_tokens + 7, f.num_tokens - t0);
+  const int owned = min(rows, p.v_tokens);
   const int chunks = f.head_dim >> 3, pitch = (chunks + 7) / 8 * 128;
   const uint16_t* src = static_cast<const uint16_t*>(p.src_v.data) + t0 * p.src_v.token_stride + head * p.src_v.head_stride;
   const uint32_t sbase = smem_u32(smem);
@@ -400,10 +410,10 @@ int launch_rotary(const RotaryArgs& a, cudaStream_t stream) {
     }
   }
   const int heads = p.hq + (a.k.data ? a.fill.num_kv_heads : 0);
-  // Eight tokens share a block once that gives every SM one; below, a token has blocks of its own, one per as many heads as
+  // Sixteen tokens share a block once that gives every SM one; below, a token has blocks of its own, one per as many heads as
   // its threads hold at once while the GPU has room for them.
   const long long sms = cached_sm_count();
-  p.block_tokens = tokens >= kTokensPerBlock * sms && half <= 768 ? kTokensPerBlock : 1;  // (their table stays within 48 KB)
+  p.block_tokens = tokens >= kTokensPerBlock * sms && half <= 384 ? kTokensPerBlock : 1;  // (their table stays within 48 KB)
   const long long groups = (tokens + p.block_tokens - 1) / p.block_tokens;
   const int units = (d + 2 * vec - 1) / (2 * vec);
   const int at_once = kThreads / units > 1 ? kThreads / units : 1;
@@ -411,9 +421,10 @@ int launch_rotary(const RotaryArgs& a, cudaStream_t stream) {
   p.head_splits = (int)(splits_room < 1 ? 1 : (splits_room < splits_wanted ? splits_room : splits_wanted));
   size_t smem = (size_t)p.block_tokens * 2 * half * sizeof(float);
   if (a.k.data) {
-    p.v_blocks = (unsigned)((tokens + kTokensPerTile - 1) / kTokensPerTile * a.fill.num_kv_heads);
+    p.v_tokens = tokens * a.fill.num_kv_heads >= kTokensPerTile * sms ? kTokensPerTile : 8;
+    p.v_blocks = (unsigned)((tokens + p.v_tokens - 1) / p.v_tokens * a.fill.num_kv_heads);
     p.v_vec = aligned_rows(a.v.data, a.v.token_stride, a.v.head_stride, 16) ? 1 : 0;
-    const size_t rows = (size_t)(tokens < kTileTokens ? tokens : kTileTokens) * ((d / 8 + 7) / 8 * 128);
+    const size_t rows = (size_t)(tokens < p.v_tokens + 7 ? tokens : p.v_tokens + 7) * ((d / 8 + 7) / 8 * 128);
     if (rows > smem) smem = rows;
   }
   const unsigned long long rotating = (unsigned long long)groups * p.head_splits;
