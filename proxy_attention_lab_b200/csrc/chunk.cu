@@ -34,10 +34,11 @@ constexpr int kMergeWarps = 4;
 // One block per (border of a share, slice of rows); a warp merges one row at a time, a lane holds 4 elements of each 128.
 // Bound: latency.  Lanes fetch the (m, l) of 32 parts at once, and four parts' rows are in flight before the first is used.
 template <typename T>
-__global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const ChunkCut* __restrict__ cuts, const float2* __restrict__ ml,
-                                                                       const float* __restrict__ acc, void* __restrict__ out, int out_f32,
+__global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const ChunkCut* cuts, const float2* ml,
+                                                                       const float* acc, void* out, int out_f32,
                                                                        int part_rows, int tile_heads, int num_q_heads, int head_dim,
                                                                        int rows_per_block) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the attention kernel runs: its results are complete from here
   const ChunkCut c = cuts[blockIdx.x];
   if (c.parts <= 1) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -108,13 +109,20 @@ int launch_chunk_merge(const ChunkArgs& a, const ChunkPlan& plan, const ChunkCut
   constexpr int kRowsPerBlock = 16;
   const dim3 grid(plan.grid, (plan.part_rows + kRowsPerBlock - 1) / kRowsPerBlock);
   const float2* ml = reinterpret_cast<const float2*>(part_ml);
-  if (a.dtype == 0)
-    chunk_merge_kernel<__half><<<grid, kMergeWarps * 32, 0, stream>>>(cuts, ml, part_acc, a.out, a.out_f32 ? 1 : 0, plan.part_rows, plan.tile_heads,
-                                                                      a.num_q_heads, a.head_dim, kRowsPerBlock);
-  else
-    chunk_merge_kernel<__nv_bfloat16><<<grid, kMergeWarps * 32, 0, stream>>>(cuts, ml, part_acc, a.out, a.out_f32 ? 1 : 0, plan.part_rows,
-                                                                             plan.tile_heads, a.num_q_heads, a.head_dim, kRowsPerBlock);
-  return (int)cudaGetLastError();
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(kMergeWarps * 32);
+  config.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  const int out_f32 = a.out_f32 ? 1 : 0;
+  return (int)(a.dtype == 0 ? cudaLaunchKernelEx(&config, chunk_merge_kernel<__half>, cuts, ml, part_acc, a.out, out_f32, plan.part_rows, plan.tile_heads,
+                                                 a.num_q_heads, a.head_dim, kRowsPerBlock)
+                            : cudaLaunchKernelEx(&config, chunk_merge_kernel<__nv_bfloat16>, cuts, ml, part_acc, a.out, out_f32, plan.part_rows,
+                                                 plan.tile_heads, a.num_q_heads, a.head_dim, kRowsPerBlock));
 }
 
 int launch_chunk(const ChunkArgs& a, cudaStream_t stream) {

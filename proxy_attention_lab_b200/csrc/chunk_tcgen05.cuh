@@ -43,8 +43,10 @@
 namespace pal {
 namespace {
 
-constexpr int kChunkItemCost = 6;    // fixed cost of an item in key tiles: query load, pipeline fill, epilogue
-constexpr int kChunkMinShare = 4;    // smallest share of a CTA, in the same unit
+// Fixed cost of an item in key tiles (query load, pipeline fill, masked tiles, output): measured 4 for an item of two tiles of
+// rows, about 2 for one of a single tile.
+constexpr int kChunkPairCost = 4, kChunkSingleCost = 2;
+constexpr int kChunkMinShare = 1;    // smallest share of a CTA, in the same unit
 constexpr int kSegRing = 4;
 
 // What one CTA does with one item: key tiles [kt0, kt1) for the rows of the item.
@@ -114,6 +116,12 @@ __device__ __forceinline__ int chunk_keys(const ChunkParams& p, const ChunkSeq& 
   return (hi + kTile - 1) / kTile - lo / kTile;
 }
 
+// Place of an item's first key tile behind its start on the line of costs.
+template <int NQ>
+__device__ __forceinline__ int chunk_item_cost(const ChunkParams& p, int tokens) {
+  return NQ == 2 && tokens > p.tile_tokens ? kChunkPairCost : kChunkSingleCost;
+}
+
 template <int D_, int TPP_, int NQ_>
 struct ChunkCfg {
   static constexpr int D = D_, TPP = TPP_, NQ = NQ_;
@@ -124,7 +132,8 @@ struct ChunkCfg {
   static constexpr int kOCol = kPCol + NQ * 64;
   static_assert(kOCol + NQ * Base::DP <= 512, "TMEM holds 512 columns");
   static constexpr int kThreads = 128 + 128 * NQ;
-  static constexpr int ST = Base::kStages;
+  // K and V ring: two tiles of each (64 KB) in flight, four where they are half as large, one of head_dim 256
+  static constexpr int ST = D <= 64 ? 4 : D <= 128 ? 2 : 1;
   static constexpr int kQ = 0;
   static constexpr int kK = NQ * Base::kTileBytes;
   static constexpr int kV = kK + ST * Base::kTileBytes;
@@ -312,23 +321,23 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBars);
   uint64_t* q_full = bars;             // 1
   uint64_t* q_empty = bars + 1;        // 1: the last QK^T of a segment has read Q
-  uint64_t* k_full = bars + 2;         // ST
-  uint64_t* k_empty = bars + 4;        // ST
-  uint64_t* v_full = bars + 6;         // ST
-  uint64_t* v_empty = bars + 8;        // ST
-  uint64_t* s_full = bars + 10;        // 2, per accumulator: its scores are in an S buffer
-  uint64_t* s_empty = bars + 28;       // 2: ... and have been read
-  uint64_t* p_full = bars + 12;        // 2: its P tile is written
-  uint64_t* o_done = bars + 14;        // 2: the PV that read it has run
-  uint64_t* merge_full = bars + 16;    // 1: the second accumulator's rows are in shared memory
-  uint64_t* merge_empty = bars + 17;   // 1
-  uint64_t* seg_done = bars + 18;      // 1: the first warpgroup has finished a segment
-  uint64_t* seg_full = bars + 20;      // kSegRing
-  uint64_t* seg_empty = bars + 24;     // kSegRing
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 30);
-  long long* sm_plan = reinterpret_cast<long long*>(bars + 32);  // scan scratch, then the share's last item
+  uint64_t* merge_full = bars + 2;     // 1: the second accumulator's rows are in shared memory
+  uint64_t* merge_empty = bars + 3;    // 1
+  uint64_t* seg_done = bars + 4;       // 1: the first warpgroup has finished a segment
+  uint64_t* s_full = bars + 6;         // 2, per accumulator: its scores are in an S buffer
+  uint64_t* s_empty = bars + 8;        // 2: ... and have been read
+  uint64_t* p_full = bars + 10;        // 2: its P tile is written
+  uint64_t* o_done = bars + 12;        // 2: the PV that read it has run
+  uint64_t* k_full = bars + 14;        // ST
+  uint64_t* k_empty = bars + 18;       // ST
+  uint64_t* v_full = bars + 22;        // ST
+  uint64_t* v_empty = bars + 26;       // ST
+  uint64_t* seg_full = bars + 30;      // kSegRing
+  uint64_t* seg_empty = bars + 34;     // kSegRing
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
+  long long* sm_plan = reinterpret_cast<long long*>(bars + 40);  // scan scratch, then the share's last item
   ChunkSegment* segs = reinterpret_cast<ChunkSegment*>(smem + C::kBars + 512);
-  static_assert(kSegRing == 4, "barrier layout");
+  static_assert(kSegRing == 4 && ST <= 4, "barrier layout");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int item_tokens = NQ * p.tile_tokens;
@@ -345,7 +354,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       const ChunkSeq q = chunk_seq(p, s, TPP);
       long long w = 0;
       int lo, hi;
-      for (int ta = 0; ta < q.n; ta += item_tokens) w += kChunkItemCost + chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi);
+      for (int ta = 0; ta < q.n; ta += item_tokens) w += chunk_item_cost<NQ>(p, q.n - ta) + chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi);
       mine += w * vheads;
     }
     long long inc = mine;
@@ -358,11 +367,13 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
     if (tid == 0) {
       mbar_init(q_full, 1);
       mbar_init(q_empty, 1);
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < ST; ++i) {
         mbar_init(&k_full[i], 32);
         mbar_init(&k_empty[i], 1);
         mbar_init(&v_full[i], 1);
         mbar_init(&v_empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[i], 1);
         mbar_init(&p_full[i], 4);
         mbar_init(&s_empty[i], 4);
@@ -405,12 +416,12 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
         const ChunkSeq q = chunk_seq(p, s, TPP);
         long long w = 0;
         int lo, hi;
-        for (int t = 0; t < q.n; t += item_tokens) w += kChunkItemCost + chunk_keys(p, q, t, min(t + item_tokens, q.n), lo, hi);
+        for (int t = 0; t < q.n; t += item_tokens) w += chunk_item_cost<NQ>(p, q.n - t) + chunk_keys(p, q, t, min(t + item_tokens, q.n), lo, hi);
         if (last < at + w * vheads) {
           vh = (int)((last - at) / w);
           at += vh * w;
           for (;; ta += item_tokens) {
-            const int c = kChunkItemCost + chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi);
+            const int c = chunk_item_cost<NQ>(p, q.n - ta) + chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi);
             if (last < at + c) break;
             at += c;
           }
@@ -463,7 +474,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       ChunkSegment g;
       g.end = 1;
       while (more && g.end) {
-        const long long first = at + kChunkItemCost;  // place of key tile 0 on the line
+        const long long first = at + chunk_item_cost<NQ>(p, q.n - ta);  // place of key tile 0 on the line
         const int t0 = (int)min((long long)nt, max(0LL, share0 - first)), t1 = (int)max(0LL, min((long long)nt, share1 - first));
         if (t1 > t0 || (nt == 0 && at >= share0)) {
           g.end = 0;
@@ -508,7 +519,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           ta = (q.n - 1) / item_tokens * item_tokens;
         }
         nt = chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi);
-        at -= kChunkItemCost + nt;
+        at -= chunk_item_cost<NQ>(p, q.n - ta) + nt;
       }
       const int slot = n_pub % kSegRing;
       if (!__all_sync(0xffffffffu, mbar_wait(&seg_empty[slot], ((n_pub / kSegRing) & 1) ^ 1, p.status))) return false;
@@ -670,14 +681,16 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
     // contiguous bytes and read two page rows.  (A TMA gather of four page rows per request brings the same tile in 2590
     // cycles, these copies in less than 1200, the turn-around of the ring it was measured with.)
     uint32_t n_seg = 0, n_tile = 0;
-    int pending = -1;  // stage whose K copies have been issued, but not yet been handed over
+    uint32_t handed = 0;  // tiles whose copies have landed and been handed over (n_tile: whose copies have been issued)
     bool ok = true;
-    auto hand_over = [&](auto keep) {  // all copies but the newest `keep` groups have landed
-      if (pending < 0) return;
-      asm volatile("cp.async.wait_group %0;" ::"n"(decltype(keep)::value) : "memory");
-      fence_proxy_async_smem();  // (read by MMAs)
-      mbar_arrive(&k_full[pending]);
-      pending = -1;
+    // hands over every tile but the newest KEEP
+    auto hand_over = [&](auto keep) {
+      constexpr uint32_t KEEP = decltype(keep)::value;
+      if (n_tile - handed <= KEEP) return;
+      asm volatile("cp.async.wait_group %0;" ::"n"(KEEP) : "memory");  // (a tile is a group of copies)
+      fence_proxy_async_smem();                                       // (read by MMAs)
+#pragma unroll 1
+      for (; n_tile - handed > KEEP; ++handed) mbar_arrive(&k_full[handed % ST]);
     };
     // a wait that may last hands over first what may be waited for
     auto wait_stage = [&](uint64_t* bar, uint32_t parity) {
@@ -710,7 +723,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
         return pid;
       };
       uint32_t next_pid = page_id(kt0);
-      for (int j = kt0; j < kt1; ++j, ++n_tile) {
+      for (int j = kt0; j < kt1; ++j) {
         const int st = n_tile % ST;
         const uint32_t pid = next_pid;
         next_pid = page_id(j + 1);
@@ -728,8 +741,8 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
               asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(k_dst + q * 512 + c * B::kChunkBytes), "l"(src + c * (TPP * 16)) : "memory");
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        hand_over(std::integral_constant<int, 1>());
-        pending = st;
+        ++n_tile;
+        hand_over(std::integral_constant<int, (ST > 2 ? ST - 1 : 1)>());
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -843,17 +856,23 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           }
           return true;
         };
-        // One tile without residual: the row in registers, straight through.  (The masked form is a copy of its own: a branch
-        // around the masking alone makes the compiler spill the scores, at twice the time of every tile.)
-        auto plain_tile = [&](auto masked, int rl, int rh) {
+        // One tile without residual: the row in registers, straight through.  (One path for masked tiles and others, and little
+        // control flow in it: masking group by group, with a branch each, made the compiler spill the scores, at twice the time
+        // of every tile; a masked copy of the path costs 5 % through the instruction cache.)
+        auto plain_tile = [&](bool masked, int rl, int rh) {
           uint32_t sc[128];
           tmem_ld128(tS, sc);
           tmem_wait_ld();
           scores_read();
-          if (decltype(masked)::value) {
+          if (masked) {
 #pragma unroll
             for (int c = 0; c < 128; ++c)
-              if (c < rl || c > rh) sc[c] = 0xff800000u;
+              if (c > rh) sc[c] = 0xff800000u;
+            if (rl > 0) {
+#pragma unroll
+              for (int c = 0; c < 128; ++c)
+                if (c < rl) sc[c] = 0xff800000u;
+            }
           }
           if (!new_max(row_max128(sc) * p.scale_log2)) return false;
           const float m_ref = m_used > -INFINITY ? m_used : 0.f;
@@ -878,10 +897,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           tmem_wait_st();  // (the score buffer now holds the residual, and is given back after the PV)
         } else {
           const int c0 = j * kTile;
-          if (c0 < all_lo || c0 + kTile - 1 > all_hi)
-            ok = plain_tile(std::true_type(), lo - c0, hi - c0);
-          else
-            ok = plain_tile(std::false_type(), 0, 0);
+          ok = plain_tile(c0 < all_lo || c0 + kTile - 1 > all_hi, lo - c0, hi - c0);
           if (!ok) break;
         }
         ++mine;
@@ -1010,6 +1026,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
 
   tc_fence_before();
   __syncthreads();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the merging kernel may start; it waits for this grid's end)
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
