@@ -43,10 +43,11 @@
 namespace pal {
 namespace {
 
-// Fixed cost of an item in key tiles (query load, pipeline fill, masked tiles, output): measured 4 for an item of two tiles of
-// rows, about 2 for one of a single tile.
-constexpr int kChunkPairCost = 4, kChunkSingleCost = 2;
-constexpr int kChunkMinShare = 1;    // smallest share of a CTA, in the same unit
+// Costs on the line of items.  A key tile for two tiles of rows is bound by the softmax (4 units); for a single one it is
+// bound by the loads of keys and values, 64 KB at head_dim 128 and half at 64 (3 and 2).  Query load, pipeline fill, masked tiles
+// and output were measured as worth four key tiles for a pair of row tiles, two for a single one.
+constexpr int kChunkMaxTileCost = 4;
+constexpr int kChunkMinShare = kChunkMaxTileCost;  // smallest share of a CTA: a whole key tile of any kind
 constexpr int kSegRing = 4;
 
 // What one CTA does with one item: key tiles [kt0, kt1) for the rows of the item.
@@ -116,10 +117,14 @@ __device__ __forceinline__ int chunk_keys(const ChunkParams& p, const ChunkSeq& 
   return (hi + kTile - 1) / kTile - lo / kTile;
 }
 
-// Place of an item's first key tile behind its start on the line of costs.
-template <int NQ>
-__device__ __forceinline__ int chunk_item_cost(const ChunkParams& p, int tokens) {
-  return NQ == 2 && tokens > p.tile_tokens ? kChunkPairCost : kChunkSingleCost;
+// The cost of an item with `tokens` tokens left in its sequence: of a key tile, and before the first.
+struct ChunkCost {
+  int tile, setup;
+};
+template <int D, int NQ>
+__device__ __forceinline__ ChunkCost chunk_cost(const ChunkParams& p, int tokens) {
+  if (NQ == 1 || tokens > p.tile_tokens) return ChunkCost{kChunkMaxTileCost, 4 * kChunkMaxTileCost};
+  return D <= 64 ? ChunkCost{2, 4} : ChunkCost{3, 6};
 }
 
 template <int D_, int TPP_, int NQ_>
@@ -159,6 +164,14 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
   return ok != 0;
+}
+
+// A wait of the MMA and softmax warps, always true: one that expires (the status word then tells) sets `dead`, later ones do not
+// last, and the warp leaves at its next segment, where all lanes look at it.  No vote and no way out of the loops in between: a
+// vote per wait cost 80 cycles each, several times per key tile.
+__device__ __forceinline__ bool chunk_wait(uint64_t* bar, uint32_t parity, const WaitCtx& ctx, bool& dead) {
+  if (!mbar_try_wait(bar, parity) && !dead) dead = !mbar_wait(bar, parity, ctx);
+  return true;
 }
 
 // tcgen05.mma with operand descriptors given as (lower, upper) halves; `accumulate` 0 starts the accumulator afresh.
@@ -219,7 +232,7 @@ __device__ __forceinline__ void chunk_exp_half(const uint32_t (&s)[128], int h, 
   }
 }
 
-// Items that feed the rounding residual take a path of their own, in rolled loops of 32 columns over the scores in place.
+// With the rounding residual tiles take a path of their own, in rolled loops of 32 columns over the scores in place.
 // Maximum over the columns in [lo, hi]:
 __device__ __forceinline__ float chunk_residual_max(uint32_t tS, int lo, int hi) {
   float m = -INFINITY;
@@ -261,14 +274,11 @@ __device__ __forceinline__ float chunk_residual_exp(uint32_t tS, uint32_t tP, in
 // 1 / l for the row sum l: 0 for a row without keys, NaN where a score was not a number
 __device__ __forceinline__ float chunk_inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
-// bf16 rounds P by up to 2^-9 of its value, which leaves about 0.002 / sqrt(n / 3) per unit of |v| over n keys.  Items with a
-// row of fewer than 256 keys, and float32 outputs, get the residual P - bf16(P) through a second set of PV MMAs.
+// bf16 rounds P by up to half a step, 2^-8, of its value: in the result no more than the rounding of a bf16 output.  A caller who
+// asks for float32 gets the residual P - bf16(P) through a second set of PV MMAs.
 template <typename T>
-__device__ __forceinline__ bool chunk_feeds_residual(const ChunkParams& p, const ChunkSegment& g) {
-  if (!Mma16816<T>::kSplitP) return false;
-  int keys = p.causal ? min(g.pos0 + 1, g.key_cap) : g.key_cap;
-  if (p.window > 0) keys = min(keys, p.window);
-  return p.out_f32 != 0 || keys < 256;
+__device__ __forceinline__ bool chunk_feeds_residual(const ChunkParams& p) {
+  return Mma16816<T>::kSplitP && p.out_f32 != 0;
 }
 
 // The 32 rows of a warp, one per lane in registers, to rows `row` (-1 = none) of `base` by way of `stage` (128 bytes per row):
@@ -341,6 +351,11 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int item_tokens = NQ * p.tile_tokens;
+  auto item_cost = [&](const ChunkSeq& q, int ta) {
+    const ChunkCost c = chunk_cost<D, NQ>(p, q.n - ta);
+    int lo, hi;
+    return c.setup + c.tile * chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi);
+  };
   const int vheads = p.num_kv_heads * p.head_blocks;
 
   // ---- the CTA's share of the line of items ----
@@ -353,8 +368,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
     for (int s = sa; s < sb; ++s) {
       const ChunkSeq q = chunk_seq(p, s, TPP);
       long long w = 0;
-      int lo, hi;
-      for (int ta = 0; ta < q.n; ta += item_tokens) w += chunk_item_cost<NQ>(p, q.n - ta) + chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi);
+      for (int ta = 0; ta < q.n; ta += item_tokens) w += item_cost(q, ta);
       mine += w * vheads;
     }
     long long inc = mine;
@@ -415,13 +429,12 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       for (; s < sb; ++s) {
         const ChunkSeq q = chunk_seq(p, s, TPP);
         long long w = 0;
-        int lo, hi;
-        for (int t = 0; t < q.n; t += item_tokens) w += chunk_item_cost<NQ>(p, q.n - t) + chunk_keys(p, q, t, min(t + item_tokens, q.n), lo, hi);
+        for (int t = 0; t < q.n; t += item_tokens) w += item_cost(q, t);
         if (last < at + w * vheads) {
           vh = (int)((last - at) / w);
           at += vh * w;
           for (;; ta += item_tokens) {
-            const int c = chunk_item_cost<NQ>(p, q.n - ta) + chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi);
+            const int c = item_cost(q, ta);
             if (last < at + c) break;
             at += c;
           }
@@ -474,8 +487,14 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       ChunkSegment g;
       g.end = 1;
       while (more && g.end) {
-        const long long first = at + chunk_item_cost<NQ>(p, q.n - ta);  // place of key tile 0 on the line
-        const int t0 = (int)min((long long)nt, max(0LL, share0 - first)), t1 = (int)max(0LL, min((long long)nt, share1 - first));
+        // a key tile belongs to the share that its place on the line starts in
+        const ChunkCost cost = chunk_cost<D, NQ>(p, q.n - ta);
+        const long long first = at + cost.setup;
+        auto tiles_before = [&](long long x) {
+          const int d = (int)min(max(x - first, 0LL), (long long)nt * cost.tile);  // (a tile count of an int32 length, times 4)
+          return (d + cost.tile - 1) / cost.tile;
+        };
+        const int t0 = tiles_before(share0), t1 = tiles_before(share1);
         if (t1 > t0 || (nt == 0 && at >= share0)) {
           g.end = 0;
           g.seq = s;
@@ -496,7 +515,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           if (t0 == 0 && t1 < nt && lane == 0) {
             // this CTA holds the item's first part: tell the merging kernel where the others are
             ChunkCut c;
-            c.parts = (int)((first + nt - 1) / share) - (int)blockIdx.x + 1;
+            c.parts = (int)((first + (long long)(nt - 1) * cost.tile) / share) - (int)blockIdx.x + 1;
             c.row0 = g.row0;
             c.tokens = g.tokens;
             c.head0 = g.head0;
@@ -519,7 +538,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           ta = (q.n - 1) / item_tokens * item_tokens;
         }
         nt = chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi);
-        at -= chunk_item_cost<NQ>(p, q.n - ta) + nt;
+        at -= item_cost(q, ta);
       }
       const int slot = n_pub % kSegRing;
       if (!__all_sync(0xffffffffu, mbar_wait(&seg_empty[slot], ((n_pub / kSegRing) & 1) ^ 1, p.status))) return false;
@@ -583,7 +602,8 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
     // before it), PV of step k when its P is there.  The two share nothing but barriers, so each has a warp: one warp that
     // issues both spends more time on the issue (8 MMAs, waits and commits: ~600 cycles each) than the MMAs take.
     constexpr int F = Fmt<T>::kCode;
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)) != 0; };
+    bool dead = false;
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return chunk_wait(bar, parity, p.status, dead); };
     auto commit = [&](uint64_t* bar) {
       if (elect_one()) tc_commit(bar);
     };
@@ -597,10 +617,10 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
     bool ok = true;
     while (ok) {
       const int slot = n_seg % kSegRing;
-      ok = wait_all(&seg_full[slot], (n_seg / kSegRing) & 1);
-      if (!ok) break;
+      wait_all(&seg_full[slot], (n_seg / kSegRing) & 1);
+      if (__any_sync(0xffffffffu, dead)) break;
       const ChunkSegment& sg = segs[slot];
-      const bool residual = uniform(chunk_feeds_residual<T>(p, sg) ? 1 : 0) != 0;
+      const bool residual = chunk_feeds_residual<T>(p);
       const int end = uniform(sg.end), kt0 = uniform(sg.kt0), num = uniform(sg.kt1) - kt0, key_lo = uniform(sg.key_lo), key_hi = uniform(sg.key_hi);
       const int pair = NQ == 2 && !uniform(sg.alternate) ? 1 : 0;
       __syncwarp();
@@ -757,13 +777,14 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
     const uint32_t lane_addr = (uint32_t)(lane_group * 32) << 16;
     const uint32_t tO = tmem_base + lane_addr + C::kOCol + wg * B::DP, tP = tmem_base + lane_addr + C::kPCol + wg * 64;
     const uint32_t tS = tmem_base + lane_addr + (NS == 2 ? wg * kTile : 0);
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status)) != 0; };
+    bool dead = false;
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return chunk_wait(bar, parity, p.status, dead); };
     uint32_t n_seg = 0, n_s = 0, n_o = 0, n_v = 0, n_merge = 0;  // segments, scores taken, PVs seen to end, key tiles, merges
     bool ok = true;
     while (ok) {
       const int slot = n_seg % kSegRing;
-      ok = wait_all(&seg_full[slot], (n_seg / kSegRing) & 1);
-      if (!ok) break;
+      wait_all(&seg_full[slot], (n_seg / kSegRing) & 1);
+      if (__any_sync(0xffffffffu, dead)) break;
       const ChunkSegment& g = segs[slot];  // (held until the segment is done: what the epilogue needs stays in shared memory)
       if (g.end) break;
       ++n_seg;
@@ -783,9 +804,11 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       const int pos_a = g.pos0 + tok_first + lane_group * 32 / p.tile_heads, pos_b = g.pos0 + tok_first + (lane_group * 32 + 31) / p.tile_heads;
       const int all_hi = p.causal ? min(pos_a, g.key_cap - 1) : g.key_cap - 1;
       const int all_lo = p.window > 0 && pos_b >= p.window ? pos_b - p.window + 1 : 0;
-      const bool residual = chunk_feeds_residual<T>(p, g);
+      const bool residual = chunk_feeds_residual<T>(p);
       float m_used = -INFINITY, l_run = 0.f;
       const int kt0 = g.kt0, num = g.kt1 - kt0;
+      // key tiles whose first or last 16-key step is only partly seen
+      const int ragged_first = g.key_lo & 15 ? g.key_lo / kTile : -1, ragged_last = g.key_hi & 15 ? g.key_hi / kTile : -1;
       int mine = 0;  // key tiles this accumulator has taken
       for (int i = 0; i < num; ++i) {
         if (alt && (i & 1) != wg) {
@@ -796,9 +819,8 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
         if (!(ok = wait_all(&s_full[wg], n_s & 1))) break;
         ++n_s;
         tc_fence_after();
-        auto scores_read = [&]() {
+        auto scores_read = [&]() {  // (behind a warp-wide tcgen05 wait)
           tc_fence_before();
-          __syncwarp();
           if (lane == 0) mbar_arrive(&s_empty[wg]);
         };
         // O and the P tile are this warp's again once the PV of the previous key tile has run
@@ -816,7 +838,6 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
         // multiplied by P = 0, which is not 0 if they hold an infinity or a NaN: zero them in the 16-key steps that are used.
         auto clear_values = [&]() {
           const int c_lo = max(0, g.key_lo - j * kTile), c_hi = min(kTile, g.key_hi - j * kTile);
-          if (!((c_lo | c_hi) & 15)) return true;
           const int st = (int)(n_v % ST);
           if (!wait_all(&v_full[st], (n_v / ST) & 1)) return false;
           unsigned char* vt = sV + st * kTileBytes;
@@ -901,7 +922,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           if (!ok) break;
         }
         ++mine;
-        if ((wg == 0 || alt) && !(ok = clear_values())) break;
+        if ((wg == 0 || alt) && (j == ragged_first || j == ragged_last) && !(ok = clear_values())) break;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[wg]);
