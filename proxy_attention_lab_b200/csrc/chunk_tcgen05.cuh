@@ -51,7 +51,7 @@ constexpr int kChunkMinShare = kChunkMaxTileCost;  // smallest share of a CTA: a
 constexpr int kSegRing = 4;
 
 // What one CTA does with one item: key tiles [kt0, kt1) for the rows of the item.
-struct ChunkSegment {
+struct ChunkWork {
   int seq, kv_head;
   int head0, heads;    // first query head of the tile, and how many of its heads exist
   int row0, tokens;    // first query row (token) and how many of the item's tokens exist
@@ -62,6 +62,13 @@ struct ChunkSegment {
   int alternate;       // one tile of rows: the accumulators take even and odd key tiles
   int slot;            // partial slot to write, -1 = the output itself
   int end;
+  // Keys that some rows of the item see and others do not: [some_hi, key_hi) at the diagonal, [key_lo, some_lo) at the start of
+  // the windows.  Each range touches at most three key tiles; `bad` marks the keys whose value is not finite.
+  int some_lo, some_hi;
+  int any_bad;
+};
+struct ChunkSegment : ChunkWork {
+  uint32_t bad[6][4];  // three tiles of the diagonal's range, three of the windows'
 };
 
 struct ChunkParams {
@@ -142,8 +149,10 @@ struct ChunkCfg {
   static constexpr int kQ = 0;
   static constexpr int kK = NQ * Base::kTileBytes;
   static constexpr int kV = kK + ST * Base::kTileBytes;
-  static constexpr int kMl = kV + ST * Base::kTileBytes;    // m, l of the second accumulator (alternate segments)
-  static constexpr int kStage = kMl + (NQ == 2 ? 1024 : 0);  // 4 KB per softmax warp on the way out
+  static constexpr int kStage = kV + ST * Base::kTileBytes;  // 4 KB per softmax warp on the way out
+  // m, l of the second accumulator in alternate segments, in which its warps store no output (and before they do in a later
+  // segment, the first warpgroup, which reads m and l, has handed over its weights there)
+  static constexpr int kMl = kStage + 4 * 4096;
   static constexpr int kBars = kStage + NQ * 4 * 4096;
   static constexpr int kUsed = kBars + 512 + kSegRing * (int)sizeof(ChunkSegment) + 1024;
   static constexpr int kTotal = kUsed < 116 * 1024 ? 116 * 1024 : kUsed;
@@ -484,7 +493,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
     // next segment of the share (the same computation on every lane), published to the other warps
     auto publish = [&]() {
       // ---- next segment of the share (the same computation on every lane) ----
-      ChunkSegment g;
+      ChunkWork g;
       g.end = 1;
       while (more && g.end) {
         // a key tile belongs to the share that its place on the line starts in
@@ -510,6 +519,9 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           g.key_lo = lo;
           g.key_hi = hi;
           g.key_cap = q.cap;
+          g.some_hi = p.causal ? max(lo, min(hi, g.pos0 + 1)) : hi;
+          g.some_lo = p.window > 0 ? min(hi, max(lo, g.pos0 + g.tokens - p.window)) : lo;
+          g.any_bad = 0;
           g.alternate = NQ == 2 && g.tokens <= p.tile_tokens;
           g.slot = t0 > 0 ? 2 * (int)blockIdx.x : (t1 < nt ? 2 * (int)blockIdx.x + 1 : -1);
           if (t0 == 0 && t1 < nt && lane == 0) {
@@ -542,8 +554,10 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       }
       const int slot = n_pub % kSegRing;
       if (!__all_sync(0xffffffffu, mbar_wait(&seg_empty[slot], ((n_pub / kSegRing) & 1) ^ 1, p.status))) return false;
+      if (lane < 24) segs[slot].bad[lane >> 2][lane & 3] = 0u;
+      __syncwarp();
       if (lane == 0) {
-        segs[slot] = g;
+        static_cast<ChunkWork&>(segs[slot]) = g;
         mbar_arrive(&seg_full[slot]);
       }
       __syncwarp();
@@ -785,7 +799,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       const int slot = n_seg % kSegRing;
       wait_all(&seg_full[slot], (n_seg / kSegRing) & 1);
       if (__any_sync(0xffffffffu, dead)) break;
-      const ChunkSegment& g = segs[slot];  // (held until the segment is done: what the epilogue needs stays in shared memory)
+      ChunkSegment& g = segs[slot];  // (held until the segment is done: what the epilogue needs stays in shared memory)
       if (g.end) break;
       ++n_seg;
       const bool alt = NQ == 2 && g.alternate;
@@ -807,8 +821,9 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       const bool residual = chunk_feeds_residual<T>(p);
       float m_used = -INFINITY, l_run = 0.f;
       const int kt0 = g.kt0, num = g.kt1 - kt0;
-      // key tiles whose first or last 16-key step is only partly seen
-      const int ragged_first = g.key_lo & 15 ? g.key_lo / kTile : -1, ragged_last = g.key_hi & 15 ? g.key_hi / kTile : -1;
+      // key tiles with values that not all rows see: up to `care_lo`, and from `care_hi` on
+      const int care_lo = g.key_lo & 15 || g.some_lo > g.key_lo ? (max(g.some_lo, g.key_lo + 1) - 1) / kTile : -1;
+      const int care_hi = g.some_hi < g.key_hi ? g.some_hi / kTile : g.key_hi & 15 ? g.key_hi / kTile : 0x7fffffff;
       int mine = 0;  // key tiles this accumulator has taken
       for (int i = 0; i < num; ++i) {
         if (alt && (i & 1) != wg) {
@@ -834,23 +849,47 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           }
           return true;
         };
-        // V rows of slots that no row of the item sees (past the last key, before the window, never written) would be
-        // multiplied by P = 0, which is not 0 if they hold an infinity or a NaN: zero them in the 16-key steps that are used.
+        // Values that a row does not see are multiplied by P = 0, which is not 0 if they hold an infinity or a NaN.  So, in the
+        // 16-key steps that are used: slots that no row of the item sees (past the last key, before the window, never written)
+        // are zeroed; a value that some rows see and others do not is zeroed if it is not finite, and its key noted: the rows
+        // that see it come out as NaN.  (Values that all rows see need no care.)
         auto clear_values = [&]() {
           const int c_lo = max(0, g.key_lo - j * kTile), c_hi = min(kTile, g.key_hi - j * kTile);
+          const int some_lo = g.some_lo - j * kTile, some_hi = g.some_hi - j * kTile;
           const int st = (int)(n_v % ST);
           if (!wait_all(&v_full[st], (n_v / ST) & 1)) return false;
           unsigned char* vt = sV + st * kTileBytes;
+          constexpr uint32_t kAbs = 0x7fff7fffu, kCarry = Mma16816<T>::kSplitP ? 0x00800080u : 0x04000400u;  // bf16, fp16
+          const int first = c_lo & ~15, last = (c_hi + 15) & ~15;  // (multiples of 8)
           for (int dr = row; dr < D; dr += 128) {
             const int sw = TPP == 16 ? ((dr >> 2) & 1) : ((dr >> 1) & 3);
-            auto clear = [&](int from, int to) {
-              for (int c = from; c < to; ++c) {
-                const int s = c % TPP;
-                *reinterpret_cast<uint16_t*>(vt + (c / TPP) * kPageBytes + dr * (TPP * 2) + ((((s >> 3) ^ sw) << 4) | ((s & 7) << 1))) = 0;
+#pragma unroll 1
+            for (int c = first; c < last; c += 8) {
+              const bool edge = c < c_lo || c + 8 > c_hi;
+              if (!edge && c >= some_lo && c + 8 <= some_hi) continue;  // seen by all rows
+              uint4* at = reinterpret_cast<uint4*>(vt + (c / TPP) * kPageBytes + dr * (TPP * 2) + ((((c % TPP) >> 3) ^ sw) << 4));
+              uint32_t w[4] = {at->x, at->y, at->z, at->w};
+              // (a magnitude with all exponent bits set carries into the sign bit)
+              const uint32_t off = (((w[0] & kAbs) + kCarry) | ((w[1] & kAbs) + kCarry) | ((w[2] & kAbs) + kCarry) | ((w[3] & kAbs) + kCarry)) & 0x80008000u;
+              if (!edge && !off) continue;
+#pragma unroll 1
+              for (int e = 0; e < 8; ++e) {
+                const int col = c + e;
+                const uint32_t mask = 0xffffu << ((e & 1) * 16);
+                const bool seen = col >= c_lo && col < c_hi;
+                const uint32_t word = e < 2 ? w[0] : e < 4 ? w[1] : e < 6 ? w[2] : w[3];
+                const bool finite = !(((word & kAbs) + kCarry) & 0x80008000u & mask);
+                if (seen && (finite || (col >= some_lo && col < some_hi))) continue;
+                if (seen) {
+                  const int key = j * kTile + col, d0 = g.some_hi / kTile;
+                  atomicOr(&g.bad[key >= g.some_hi ? j - d0 : 3 + j - g.key_lo / kTile][col >> 5], 1u << (col & 31));
+                  g.any_bad = 1;
+                }
+                const uint32_t kept = word & ~mask;
+                if (e < 2) w[0] = kept; else if (e < 4) w[1] = kept; else if (e < 6) w[2] = kept; else w[3] = kept;
               }
-            };
-            clear(c_lo & ~15, c_lo);
-            clear(c_hi, (c_hi + 15) & ~15);
+              *at = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
           fence_proxy_async_smem();
           return true;
@@ -922,7 +961,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           if (!ok) break;
         }
         ++mine;
-        if ((wg == 0 || alt) && (j == ragged_first || j == ragged_last) && !(ok = clear_values())) break;
+        if ((wg == 0 || alt) && (j <= care_lo || j >= care_hi) && !(ok = clear_values())) break;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[wg]);
@@ -945,6 +984,19 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       tc_fence_after();
       const bool any = mine > 0 && m_used > -INFINITY;
       float m_row = any ? m_used : -INFINITY, l_row = any ? l_run : 0.f;
+      auto poisoned = [&]() {  // this row sees a key whose value is not finite
+        bool bad = false;
+#pragma unroll 1
+        for (int k = 0; k < 24; ++k) {
+          const uint32_t word = g.bad[k >> 2][k & 3];
+          const int key0 = ((k < 12 ? g.some_hi / kTile : g.key_lo / kTile - 3) + (k >> 2)) * kTile + (k & 3) * 32;
+          for (uint32_t left = word; left; left &= left - 1) {
+            const int key = key0 + __ffs(left) - 1;
+            bad = bad || (key >= lo && key <= hi);
+          }
+        }
+        return bad;
+      };
       float w_own = any ? 1.f : 0.f, w_other = 0.f;
       const int used_rows = tile_tokens * p.tile_heads;
       const bool merge = alt && num > 1;  // with a single key tile the second accumulator has nothing
@@ -990,6 +1042,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
               l_row = l_row * w_own + ml.y * w_other;
               m_row = m;
             }
+            if (g.any_bad && poisoned()) l_row = __int_as_float(0x7fffffff);
             const bool direct = g.slot < 0;
             const float inv = direct ? chunk_inverse_sum(l_row) : 1.f;
             const float f0 = w_own * inv, f1 = w_other * inv;

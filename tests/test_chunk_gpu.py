@@ -284,3 +284,52 @@ def test_refusals(pal, cuda):
     odd = torch.zeros((3, 2, 48, 16), dtype=BF16, device=cuda)
     with pytest.raises(RuntimeError, match="no kernel"):
         call(q[..., :48].contiguous(), torch.zeros((3, 2, 6, 16, 8), dtype=BF16, device=cuda), odd, t, l, cu)
+
+
+def _poison(case, s, token, value, keys=True, dims=slice(None)):
+    """Put `value` into a token of sequence s."""
+    tpp = case["v_pool"].shape[3]
+    page, slot = int(case["table"][s, token // tpp]), token % tpp
+    if keys:
+        case["k_pool"][page, :, :, slot] = value
+    case["v_pool"][page, :, dims, slot] = value
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("hq,hkv,d,tpp", [(8, 2, 128, 16), (2, 2, 64, 32), (4, 1, 256, 16), (3, 1, 80, 32)])
+def test_values_a_row_does_not_see_do_not_reach_it(pal, cuda, dtype, value, hq, hkv, d, tpp):
+    """A token that is not finite: the rows before it, and those whose window starts after it, are untouched."""
+    new, lens = [300, 5, 40], [430, 900, 40]
+    for window in (None, 150):
+        case = make_chunk_case(31, new, lens, hq, hkv, d, tpp=tpp, dtype=dtype, device=cuda, window=window)
+        clean = _run(pal, case).clone()
+        # (sequence, token, only values or keys too, which elements)
+        spots = [(0, 130 + 77, False, slice(3, 4)), (0, 429, True, slice(None)), (1, 898, False, slice(None)), (2, 17, False, slice(0, 1))]
+        if window:
+            spots.append((0, 130 - 100, False, slice(5, 7)))  # seen by the first rows, then left behind
+        for s, token, keys, dims in spots:
+            _poison(case, s, token, value, keys, dims)
+        out = _run(pal, case)
+        row0 = 0
+        for s, (n, L) in enumerate(zip(new, lens)):
+            pos = torch.arange(L - n, L, device=cuda)
+            sees = torch.zeros(n, dtype=torch.bool, device=cuda)
+            for s2, token, _, _ in spots:
+                if s2 == s:
+                    sees |= (pos >= token) & ((pos - token < window) if window else True)
+            rows, before = out[row0:row0 + n], clean[row0:row0 + n]
+            # the same arithmetic on what they see: bit for bit
+            assert torch.equal(rows[~sees].view(torch.int16), before[~sees].view(torch.int16)), (window, s)
+            if bool(sees.any()):
+                assert not torch.isfinite(rows[sees].float()).all(-1).any(), (window, s)
+            row0 += n
+        assert 0 < int((~torch.isfinite(out.float()).all(-1)).any(-1).sum()) < sum(new)
+
+
+def test_float32_output_with_a_value_that_is_not_finite(pal, cuda):
+    case = make_chunk_case(32, [100], [400], 8, 2, 128, dtype=BF16, device=cuda)
+    clean = _run(pal, case, out_dtype=torch.float32).clone()
+    _poison(case, 0, 350, float("inf"))
+    out = _run(pal, case, out_dtype=torch.float32)
+    assert torch.equal(out[:50], clean[:50]) and not torch.isfinite(out[50:]).all(-1).any()
