@@ -342,7 +342,6 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
   uint64_t* q_empty = bars + 1;        // 1: the last QK^T of a segment has read Q
   uint64_t* merge_full = bars + 2;     // 1: the second accumulator's rows are in shared memory
   uint64_t* merge_empty = bars + 3;    // 1
-  uint64_t* seg_done = bars + 4;       // 1: the first warpgroup has finished a segment
   uint64_t* s_full = bars + 6;         // 2, per accumulator: its scores are in an S buffer
   uint64_t* s_empty = bars + 8;        // 2: ... and have been read
   uint64_t* p_full = bars + 10;        // 2: its P tile is written
@@ -404,7 +403,6 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       }
       mbar_init(merge_full, 4);
       mbar_init(merge_empty, 4);
-      mbar_init(seg_done, 4);
       for (int i = 0; i < kSegRing; ++i) {
         mbar_init(&seg_full[i], 1);
         mbar_init(&seg_empty[i], 3 + 4 * NQ);
@@ -575,7 +573,9 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       // alternate segments ----
       if (lane == 0) {
         ok = mbar_wait(q_empty, (n_seg & 1) ^ 1, p.status);
-        if (ok && !alternate && prev_alternate) ok = mbar_wait(seg_done, (n_seg & 1) ^ 1, p.status);
+        // (QK^T runs up to two segments ahead of the softmax, so a barrier that counts segments could be two phases behind
+        // and its parity mistaken; the previous segment's slot cannot be released twice before its ring comes round)
+        if (ok && !alternate && prev_alternate) ok = mbar_wait(&seg_empty[(n_seg - 1) % kSegRing], ((n_seg - 1) / kSegRing) & 1, p.status);
         if (ok && kt0 < kt1) {
           const int tiles = NQ == 2 && !alternate ? 2 : 1;
           mbar_arrive_expect_tx(q_full, tiles * kBlocks * p.tile_heads * p.tile_tokens * 128);
@@ -1091,10 +1091,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       tc_fence_before();
       if (alt) fence_proxy_async_smem();  // the merge buffer's next user may be a TMA load
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&seg_empty[slot]);
-        if (wg == 0) mbar_arrive(seg_done);
-      }
+      if (lane == 0) mbar_arrive(&seg_empty[slot]);
     }
   }
 

@@ -116,6 +116,21 @@ def test_many_short_sequences(pal, cuda):
     assert_chunk(_run(pal, case), case)
 
 
+@pytest.mark.parametrize("d,tpp", [(32, 16), (64, 16), (64, 32), (96, 32), (128, 16)])
+@pytest.mark.parametrize("hq,hkv", [(32, 8), (12, 4), (16, 16)])
+def test_items_of_one_and_two_row_tiles_in_turn(pal, cuda, d, tpp, hq, hkv):
+    """Rows that fill one tile or part of it (their two accumulators are merged in the second query tile's place) between items
+    of two tiles, of one, two and more key tiles: a tile of queries is not loaded before the merge in its place has been read."""
+    g = torch.Generator().manual_seed(d + hq)
+    pick = lambda values, n: [values[int(i)] for i in torch.randint(0, len(values), (n,), generator=g)]
+    for dtype in (BF16, FP16):
+        new = pick([1, 1, 5, 20, 91, 130, 260], 48)
+        lens = [n + h for n, h in zip(new, pick([0, 17, 130, 260, 900], 48))]
+        case = make_chunk_case(d, new, lens, hq, hkv, d, tpp=tpp, dtype=dtype, device=cuda)
+        for _ in range(4):
+            assert_chunk(_run(pal, case), case)
+
+
 def test_scale_and_large_scores(pal, cuda):
     """Scores of hundreds: the running maximum moves, and single keys take all the weight."""
     case = make_chunk_case(15, [100, 2], [800, 1500], 8, 2, 128, dtype=BF16, device=cuda, q_scale=20.0)
