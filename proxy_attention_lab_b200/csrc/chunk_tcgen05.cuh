@@ -819,7 +819,9 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       const int all_hi = p.causal ? min(pos_a, g.key_cap - 1) : g.key_cap - 1;
       const int all_lo = p.window > 0 && pos_b >= p.window ? pos_b - p.window + 1 : 0;
       const bool residual = chunk_feeds_residual<T>(p);
-      float m_used = -INFINITY, l_run = 0.f;
+      // (rows that do not exist hold other tokens' queries or whatever was there: with an infinite maximum they never ask for a
+      // rescaling, whose rounding would differ from call to call)
+      float m_used = row_exists ? -INFINITY : INFINITY, l_run = 0.f;
       const int kt0 = g.kt0, num = g.kt1 - kt0;
       // key tiles with values that not all rows see: up to `care_lo`, and from `care_hi` on
       const int care_lo = g.key_lo & 15 || g.some_lo > g.key_lo ? (max(g.some_lo, g.key_lo + 1) - 1) / kTile : -1;

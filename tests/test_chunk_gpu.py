@@ -183,6 +183,20 @@ def test_repeated_calls_agree_bit_for_bit(pal, cuda):
         assert torch.equal(_run(pal, case).view(torch.int16), first.view(torch.int16))
 
 
+@pytest.mark.parametrize("d,tpp", [(32, 16), (64, 32), (128, 16), (256, 16)])
+@pytest.mark.parametrize("hq,hkv", [(12, 4), (14, 2), (8, 8)])
+def test_rows_of_a_tile_that_do_not_exist_change_nothing(pal, cuda, d, tpp, hq, hkv):
+    """Three heads per kv head leave two rows of a tile unused, seven leave two, and short items more: bit for bit the same
+    results whatever stands there, and whatever the calls before left in shared memory."""
+    new, lens = [260, 91, 130, 5, 43] * 8, [1160, 91, 260, 400, 43] * 8
+    case = make_chunk_case(d, new, lens, hq, hkv, d, tpp=tpp, dtype=BF16, device=cuda)
+    other = make_chunk_case(d + 1, [200] * 64, [300] * 64, hq, hkv, d, tpp=tpp, dtype=BF16, device=cuda, q_scale=50.0)
+    out = _run(pal, case).clone()
+    for _ in range(6):
+        _run(pal, other)
+        assert torch.equal(out, _run(pal, case))
+
+
 def test_agrees_with_decode_and_prefill(pal, cuda):
     """One token per sequence is the decode step; a chunk is the prefill with the same keys appended first."""
     case = make_chunk_case(20, [1] * 6, [300, 1, 2000, 17, 128, 900], 32, 8, 128, dtype=BF16, device=cuda)
