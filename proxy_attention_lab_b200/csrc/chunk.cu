@@ -32,8 +32,12 @@ namespace {
 constexpr int kMergeWarps = 4;
 
 // One block per (border of a share, slice of rows); a warp merges one row at a time, a lane holds 4 elements of each 128.
-// Bound: latency.  Lanes fetch the (m, l) of 32 parts at once, and four parts' rows are in flight before the first is used.
-template <typename T>
+// Bound: latency.  What a row needs is asked for at once: lanes fetch the (m, l) of 32 parts, one each, and the rows of the
+// first eight parts are on the way before the weights are known; few rows need a second trip.  (5 tokens over 1000, 32 / 8 heads of
+// 128, eight parts an item: 16.6 us a call, of which 4 in this kernel; four rows a warp, each part asked for when its weight is
+// known: 23.5.)
+constexpr int kMergeParts = 8;
+template <typename T, int NV>  // NV: pieces of 128 elements of a row
 __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const ChunkCut* cuts, const float2* ml,
                                                                        const float* acc, void* out, int out_f32,
                                                                        int part_rows, int tile_heads, int num_q_heads, int head_dim,
@@ -47,35 +51,40 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const Chu
   for (int r = blockIdx.y * rows_per_block + warp; r < r_end; r += kMergeWarps) {
     const int tok = r / tile_heads, head = r - tok * tile_heads;
     if (head >= c.heads) continue;
-    float m = -INFINITY;
-    for (int k = lane; k < c.parts; k += 32) m = fmaxf(m, ml[(size_t)slot_of(k) * part_rows + r].x);
+    float4 y[kMergeParts][NV];
+    auto fetch = [&](int k0) {  // parts k0 .. of this row
+#pragma unroll
+      for (int u = 0; u < kMergeParts; ++u)
+        if (k0 + u < c.parts)
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+            if (i * 128 + lane * 4 < head_dim)
+              y[u][i] = *reinterpret_cast<const float4*>(acc + ((size_t)slot_of(k0 + u) * part_rows + r) * head_dim + i * 128 + lane * 4);
+    };
+    auto stats = [&](int k) { return k < c.parts ? ml[(size_t)slot_of(k) * part_rows + r] : make_float2(-INFINITY, 0.f); };
+    const float2 first = stats(lane);
+    fetch(0);
+    float m = first.x;
+    for (int k = lane + 32; k < c.parts; k += 32) m = fmaxf(m, stats(k).x);
 #pragma unroll
     for (int sh = 16; sh >= 1; sh >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, sh));
     float den = 0.f;
-    float4 x[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};  // head_dim up to 256
+    float4 x[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k0 = 0; k0 < c.parts; k0 += 32) {
-      float w = 0.f;
-      if (k0 + lane < c.parts) {
-        const float2 v = ml[(size_t)slot_of(k0 + lane) * part_rows + r];
-        w = v.x > -INFINITY ? fast_exp2(v.x - m) : 0.f;
-        den += v.y * w;
-      }
+      const float2 v = k0 == 0 ? first : stats(k0 + lane);
+      const float w = v.x > -INFINITY ? fast_exp2(v.x - m) : 0.f;
+      den += v.y * w;
       const int count = min(32, c.parts - k0);
-      for (int j = 0; j < count; j += 4) {
-        float4 y[4][2];
+      for (int j = 0; j < count; j += kMergeParts) {
+        if (k0 + j > 0) fetch(k0 + j);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (j + u < count)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (i * 128 + lane * 4 < head_dim)
-                y[u][i] = *reinterpret_cast<const float4*>(acc + ((size_t)slot_of(k0 + j + u) * part_rows + r) * head_dim + i * 128 + lane * 4);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < kMergeParts; ++u) {
           const float wu = __shfl_sync(0xffffffffu, w, (j + u) & 31);
           if (j + u < count && wu != 0.f)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < NV; ++i)
               if (i * 128 + lane * 4 < head_dim) {
                 x[i].x = fmaf(y[u][i].x, wu, x[i].x);
                 x[i].y = fmaf(y[u][i].y, wu, x[i].y);
@@ -90,7 +99,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const Chu
     const float inv = den == 0.f ? 0.f : 1.f / den;
     const size_t o = ((size_t)(c.row0 + tok) * num_q_heads + c.head0 + head) * head_dim;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NV; ++i) {
       const int d = i * 128 + lane * 4;
       if (d >= head_dim) continue;
       if (out_f32)
@@ -106,11 +115,11 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const Chu
 
 int launch_chunk_merge(const ChunkArgs& a, const ChunkPlan& plan, const ChunkCut* cuts, const float* part_ml, const float* part_acc,
                        cudaStream_t stream) {
-  constexpr int kRowsPerBlock = 16;
-  const dim3 grid(plan.grid, (plan.part_rows + kRowsPerBlock - 1) / kRowsPerBlock);
-  const float2* ml = reinterpret_cast<const float2*>(part_ml);
+  // a row a warp up to 64 rows, up to four rows a warp above: sixteen blocks of 128 threads for each SM run at once
+  const int slices = min((plan.part_rows + kMergeWarps - 1) / kMergeWarps, 16);
+  const int rows_per_block = (plan.part_rows + slices - 1) / slices;
   cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
+  config.gridDim = dim3(plan.grid, slices);
   config.blockDim = dim3(kMergeWarps * 32);
   config.stream = stream;
   cudaLaunchAttribute attr;
@@ -118,11 +127,12 @@ int launch_chunk_merge(const ChunkArgs& a, const ChunkPlan& plan, const ChunkCut
   attr.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attr;
   config.numAttrs = 1;
-  const int out_f32 = a.out_f32 ? 1 : 0;
-  return (int)(a.dtype == 0 ? cudaLaunchKernelEx(&config, chunk_merge_kernel<__half>, cuts, ml, part_acc, a.out, out_f32, plan.part_rows, plan.tile_heads,
-                                                 a.num_q_heads, a.head_dim, kRowsPerBlock)
-                            : cudaLaunchKernelEx(&config, chunk_merge_kernel<__nv_bfloat16>, cuts, ml, part_acc, a.out, out_f32, plan.part_rows,
-                                                 plan.tile_heads, a.num_q_heads, a.head_dim, kRowsPerBlock));
+  auto launch = [&](auto kernel) {
+    return (int)cudaLaunchKernelEx(&config, kernel, cuts, reinterpret_cast<const float2*>(part_ml), part_acc, a.out, a.out_f32 ? 1 : 0, plan.part_rows,
+                                   plan.tile_heads, a.num_q_heads, a.head_dim, rows_per_block);
+  };
+  if (a.head_dim <= 128) return a.dtype == 0 ? launch(chunk_merge_kernel<__half, 1>) : launch(chunk_merge_kernel<__nv_bfloat16, 1>);
+  return a.dtype == 0 ? launch(chunk_merge_kernel<__half, 2>) : launch(chunk_merge_kernel<__nv_bfloat16, 2>);
 }
 
 int launch_chunk(const ChunkArgs& a, cudaStream_t stream) {
