@@ -984,8 +984,10 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
         if (!ok) break;
       }
       tc_fence_after();
-      const bool any = mine > 0 && m_used > -INFINITY;
-      float m_row = any ? m_used : -INFINITY, l_row = any ? l_run : 0.f;
+      // (a row whose keys here are all NaN has no maximum, but a sum that is not a number: it counts)
+      const bool nan = mine > 0 && l_run != l_run;
+      const bool any = mine > 0 && (m_used > -INFINITY || nan);
+      float m_row = any ? (nan ? fmaxf(m_used, 0.f) : m_used) : -INFINITY, l_row = any ? l_run : 0.f;
       auto poisoned = [&]() {  // this row sees a key whose value is not finite
         bool bad = false;
 #pragma unroll 1

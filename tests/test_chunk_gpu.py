@@ -356,6 +356,23 @@ def test_values_a_row_does_not_see_do_not_reach_it(pal, cuda, dtype, value, hq, 
         assert 0 < int((~torch.isfinite(out.float()).all(-1)).any(-1).sum()) < sum(new)
 
 
+@pytest.mark.parametrize("d,tpp", [(64, 16), (128, 32), (256, 16)])
+@pytest.mark.parametrize("length", [1, 33, 129, 300])
+def test_keys_that_are_not_numbers(pal, cuda, d, tpp, length):
+    """A row that sees a NaN key is NaN, be it the only key, the only one of its tile or of a part of the tile, or one of many."""
+    for new in (1, 40):
+        if new > length:
+            continue
+        for first in {0, length // 2, length - 1}:
+            case = make_chunk_case(33, [new], [length], 8, 2, d, tpp=tpp, dtype=BF16, device=cuda)
+            clean = _run(pal, case).clone()
+            for token in range(first, length):
+                _poison(case, 0, token, float("nan"))
+            out = _run(pal, case)
+            sees = torch.arange(length - new, length, device=cuda) >= first
+            assert torch.isnan(out[sees]).all() and torch.equal(out[~sees], clean[~sees])
+
+
 def test_float32_output_with_a_value_that_is_not_finite(pal, cuda):
     case = make_chunk_case(32, [100], [400], 8, 2, 128, dtype=BF16, device=cuda)
     clean = _run(pal, case, out_dtype=torch.float32).clone()
