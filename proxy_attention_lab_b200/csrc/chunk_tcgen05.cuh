@@ -45,7 +45,9 @@ namespace {
 
 // Costs on the line of items.  A key tile for two tiles of rows is bound by the softmax (4 units); for a single one it is
 // bound by the loads of keys and values, 64 KB at head_dim 128 and half at 64 (3 and 2).  Query load, pipeline fill, masked tiles
-// and output were measured as worth four key tiles for a pair of row tiles, two for a single one.
+// and output come on top: four key tiles' worth for a pair of row tiles, five to six for a single one.  (45 single tokens over
+// 64 to 6000, 16 heads of 64: 209 us with two for a single one, CTAs with many short items then end at 187 us and the median at
+// 123; 160-166 us with five or six.  The same over 8 heads of 128: 139 and 125.)
 constexpr int kChunkMaxTileCost = 4;
 constexpr int kChunkMinShare = kChunkMaxTileCost;  // smallest share of a CTA: a whole key tile of any kind
 constexpr int kSegRing = 4;
@@ -131,7 +133,7 @@ struct ChunkCost {
 template <int D, int NQ>
 __device__ __forceinline__ ChunkCost chunk_cost(const ChunkParams& p, int tokens) {
   if (NQ == 1 || tokens > p.tile_tokens) return ChunkCost{kChunkMaxTileCost, 4 * kChunkMaxTileCost};
-  return D <= 64 ? ChunkCost{2, 4} : ChunkCost{3, 6};
+  return D <= 64 ? ChunkCost{2, 12} : ChunkCost{3, 14};
 }
 
 template <int D_, int TPP_, int NQ_>
