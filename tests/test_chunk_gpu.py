@@ -379,3 +379,27 @@ def test_float32_output_with_a_value_that_is_not_finite(pal, cuda):
     _poison(case, 0, 350, float("inf"))
     out = _run(pal, case, out_dtype=torch.float32)
     assert torch.equal(out[:50], clean[:50]) and not torch.isfinite(out[50:]).all(-1).any()
+
+
+def test_pages_beyond_32_bit_offsets(pal, cuda):
+    """Pages whose elements lie past 2^32 bytes and 2^31 elements of the pools: append with rotation, then attend, as in a small pool."""
+    hq, hkv, d, tpp, n = 8, 8, 128, 16, 40
+    pages = 2 ** 31 // (hkv * d * tpp) + 64
+    g = torch.Generator().manual_seed(41)
+    rand = lambda *shape: torch.randn(shape, generator=g).to(BF16).to(cuda)
+    keys, values, queries = rand(n, hkv, d), rand(n, hkv, d), rand(n, hq, d)
+    inv_freq = (10000.0 ** -(torch.arange(d // 2, dtype=torch.float64) / (d // 2))).float().to(cuda)
+    pos = torch.arange(n, dtype=torch.int32, device=cuda)
+    seq = torch.zeros(n, dtype=torch.int32, device=cuda)
+    lens = torch.tensor([n], dtype=torch.int32, device=cuda)
+    outs = []
+    for total, ids in ((4, [2, 0, 3]), (pages, [pages - 1, 5, pages - 40])):
+        k = torch.zeros((total, hkv, d // 8, tpp, 8), dtype=BF16, device=cuda)
+        v = torch.zeros((total, hkv, d, tpp), dtype=BF16, device=cuda)
+        table = torch.tensor([ids], dtype=torch.int32, device=cuda)
+        _, _, q = pal.fill_kv_pages_rotary(keys, values, k, v, table, pos, seq, inv_freq=inv_freq, queries=queries)
+        outs.append((k[ids].clone(), v[ids].clone(), pal.paged_attention_chunk(q, k, v, table, lens)))
+        del k, v
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    assert outs[0][2].abs().sum() > 0
