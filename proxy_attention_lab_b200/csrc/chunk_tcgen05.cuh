@@ -152,16 +152,16 @@ struct ChunkCfg {
   static constexpr int kK = NQ * Base::kTileBytes;
   static constexpr int kV = kK + ST * Base::kTileBytes;
   static constexpr int kStage = kV + ST * Base::kTileBytes;  // 4 KB per softmax warp on the way out
-  // m, l of the second accumulator in alternate segments, in which its warps store no output (and before they do in a later
-  // segment, the first warpgroup, which reads m and l, has handed over its weights there)
-  static constexpr int kMl = kStage + 4 * 4096;
-  static constexpr int kBars = kStage + NQ * 4 * 4096;
-  static constexpr int kUsed = kBars + 512 + kSegRing * (int)sizeof(ChunkSegment) + 1024;
-  static constexpr int kTotal = kUsed < 116 * 1024 ? 116 * 1024 : kUsed;
   // the second Q tile as a buffer of fp32 rows: 16-byte pieces per row (whole groups of eight) and rows that fit
   static constexpr int kMergePitch = (D / 4 + 7) / 8 * 8;
   static constexpr int kMergeRows = Base::kTileBytes / (16 * kMergePitch) < 128 ? 64 : 128;
   static_assert(kMergeRows * kMergePitch * 16 <= Base::kTileBytes, "merge buffer");
+  // m, l of the rows in that buffer.  They have a place of their own: the second accumulator's warps may be segments ahead of the
+  // reader (a pair of row tiles without keys waits for nothing) and store their output through the stage there.
+  static constexpr int kMl = kStage + NQ * 4 * 4096;
+  static constexpr int kBars = kMl + (NQ == 2 ? kMergeRows * 8 : 0);
+  static constexpr int kUsed = kBars + 512 + kSegRing * (int)sizeof(ChunkSegment) + 1024;
+  static constexpr int kTotal = kUsed < 116 * 1024 ? 116 * 1024 : kUsed;
 };
 
 // Has the phase completed?  Never suspends the thread (mbar_try_wait may, for microseconds).
@@ -1016,7 +1016,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           if (!(ok = wait_all(merge_empty, (n_merge & 1) ^ 1))) break;
           ++n_merge;
           if (row / C::kMergeRows == pass && lane_group * 32 < used_rows) {
-            sMl[row] = make_float2(m_row, l_row);
+            sMl[row % C::kMergeRows] = make_float2(m_row, l_row);
 #pragma unroll 1
             for (int c = 0; c < D / kOC; ++c) {
               uint32_t v[kOC];
@@ -1041,7 +1041,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           }
           if ((!merge || row / C::kMergeRows == pass) && lane_group * 32 < used_rows) {
             if (merge) {
-              const float2 ml = sMl[row];
+              const float2 ml = sMl[row % C::kMergeRows];
               const float m = fmaxf(m_row, ml.x);
               w_own = m_row > -INFINITY ? fast_exp2(m_row - m) : 0.f;
               w_other = ml.x > -INFINITY ? fast_exp2(ml.x - m) : 0.f;

@@ -90,6 +90,21 @@ def test_rows_without_keys_are_zero(pal, cuda):
     assert not out[:5].any() and not out[5:5 + 50].any() and out[55:75].any()
 
 
+@pytest.mark.parametrize("d,tpp", [(32, 32), (64, 16), (64, 32), (80, 16), (128, 16), (256, 16)])
+@pytest.mark.parametrize("out_dtype", [None, torch.float32])
+def test_rows_without_keys_leave_their_neighbours_alone(pal, cuda, d, tpp, out_dtype):
+    """Sequences without keys, of rows for two row tiles, each before a short one whose key tiles (three, or six) are shared by the
+    two accumulators: the zeros of the former go out while the latter's accumulators meet."""
+    for new, lens, hq, hkv in (([64, 1] * 64, [0, 300] * 64, 32, 8), ([64, 4] * 32, [0, 300] * 32, 32, 8), ([300, 2] * 40, [0, 700] * 40, 8, 2)):
+        case = make_chunk_case(d + len(new), new, lens, hq, hkv, d, tpp=tpp, dtype=BF16, device=cuda)
+        case["out_dtype"] = out_dtype
+        empty = torch.cat([torch.full((n,), L == 0) for n, L in zip(new, lens)]).to(cuda)
+        for _ in range(3):
+            out = _run(pal, case, out_dtype=out_dtype)
+            assert_chunk(out, case)
+            assert not out[empty].any()
+
+
 def test_no_pages_and_no_rows(pal, cuda):
     q = torch.randn((3, 4, 128), device=cuda).to(BF16)
     k = torch.empty((0, 2, 16, 16, 8), dtype=BF16, device=cuda)
