@@ -43,13 +43,15 @@
 namespace pal {
 namespace {
 
-// Costs on the line of items.  A key tile for two tiles of rows is bound by the softmax (4 units); for a single one it is
-// bound by the loads of keys and values, 64 KB at head_dim 128 and half at 64 (3 and 2).  Query load, pipeline fill, masked tiles
-// and output come on top: four key tiles' worth for a pair of row tiles, five to six for a single one.  (45 single tokens over
-// 64 to 6000, 16 heads of 64: 209 us with two for a single one, CTAs with many short items then end at 187 us and the median at
-// 123; 160-166 us with five or six.  The same over 8 heads of 128: 139 and 125.)
-constexpr int kChunkMaxTileCost = 4;
-constexpr int kChunkMinShare = kChunkMaxTileCost;  // smallest share of a CTA: a whole key tile of any kind
+// Costs on the line of items, in quarters of a key tile for two tiles of rows (560 ns of a CTA's time at head_dim 128).  Such a
+// tile is bound by the softmax (4 units); for a single one it is bound by the loads of keys and values, 64 KB at head_dim 128 and
+// half at 64 (3 and 2).  Tiles with the residual of P hold their score buffer until their PV has run: 512 rows a sequence over
+// 8192 keys take 3.4 to 3.8 times as long with it at head_dim 80 to 128 (one score buffer; 14), 2.0 at 32 and 64 (two; 8), 1.6 at 256
+// (7); single tiles of rows 2.2 to 2.5 and 1.6 to 1.8 times (7 and 4).  Query load, pipeline fill, masked tiles and output come on
+// top: four key tiles' worth for a pair of row tiles, five to six for a single one.  (45 single tokens over 64 to 6000, 16 heads
+// of 64: 209 us with two for a single one, CTAs with many short items then end at 187 us and the median at 123; 160-166 us with
+// five or six.  The same over 8 heads of 128: 139 and 125.  The constants of the other head sizes follow these two.)
+constexpr int kChunkMinShare = 4;  // smallest share of a CTA; it also holds a whole key tile of every kind that occurs
 constexpr int kSegRing = 4;
 
 // What one CTA does with one item: key tiles [kt0, kt1) for the rows of the item.
@@ -62,6 +64,7 @@ struct ChunkWork {
   int key_lo, key_hi;  // keys that some row of the item sees
   int key_cap;         // keys of the sequence
   int alternate;       // one tile of rows: the accumulators take even and odd key tiles
+  int residual;        // the rounding residual of P takes part
   int slot;            // partial slot to write, -1 = the output itself
   int end;
   // Keys that some rows of the item see and others do not: [some_hi, key_hi) at the diagonal, [key_lo, some_lo) at the start of
@@ -126,14 +129,29 @@ __device__ __forceinline__ int chunk_keys(const ChunkParams& p, const ChunkSeq& 
   return (hi + kTile - 1) / kTile - lo / kTile;
 }
 
-// The cost of an item with `tokens` tokens left in its sequence: of a key tile, and before the first.
+// bf16 rounds P by up to half a step, 2^-8, of its value.  The sum over many keys averages that out; a row of few keys shows it, in
+// a bf16 result too: below 256 keys results miss 2e-3 and one unit in the last place (single tokens over 2 to 16 keys, 32 heads of
+// 128: one element in 3000).  So an item one of whose rows sees fewer than 256 keys gets the residual P - bf16(P) through a second
+// set of PV MMAs, as in the prefill kernel, and every item of a caller who asks for float32.  (For every item of one tile of rows:
+// 64 times 4 tokens over 1024 to 4096 take 317 us instead of 156.)  `ta`: the item's first token, which sees the fewest keys.
+constexpr int kResidualKeys = 256;
+template <typename T>
+__device__ __forceinline__ bool chunk_feeds_residual(const ChunkParams& p, const ChunkSeq& q, int ta) {
+  if (!Mma16816<T>::kSplitP) return false;
+  const int keys = p.causal ? min(q.len - q.n + ta + 1, q.cap) : q.cap;
+  return p.out_f32 != 0 || (p.window > 0 ? min(keys, p.window) : keys) < kResidualKeys;
+}
+
+// The cost of the item that starts at token `ta` of its sequence: of a key tile, and before the first.
 struct ChunkCost {
   int tile, setup;
 };
-template <int D, int NQ>
-__device__ __forceinline__ ChunkCost chunk_cost(const ChunkParams& p, int tokens) {
-  if (NQ == 1 || tokens > p.tile_tokens) return ChunkCost{kChunkMaxTileCost, 4 * kChunkMaxTileCost};
-  return D <= 64 ? ChunkCost{2, 12} : ChunkCost{3, 14};
+template <typename T, int D, int NQ>
+__device__ __forceinline__ ChunkCost chunk_cost(const ChunkParams& p, const ChunkSeq& q, int ta) {
+  const bool residual = chunk_feeds_residual<T>(p, q, ta);
+  if (NQ == 1) return ChunkCost{residual ? 7 : 4, 16};
+  if (q.n - ta > p.tile_tokens) return ChunkCost{residual ? (D <= 64 ? 8 : 14) : 4, 16};
+  return D <= 64 ? ChunkCost{residual ? 4 : 2, 12} : ChunkCost{residual ? 7 : 3, 14};
 }
 
 template <int D_, int TPP_, int NQ_>
@@ -285,13 +303,6 @@ __device__ __forceinline__ float chunk_residual_exp(uint32_t tS, uint32_t tP, in
 // 1 / l for the row sum l: 0 for a row without keys, NaN where a score was not a number
 __device__ __forceinline__ float chunk_inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
-// bf16 rounds P by up to half a step, 2^-8, of its value: in the result no more than the rounding of a bf16 output.  A caller who
-// asks for float32 gets the residual P - bf16(P) through a second set of PV MMAs.
-template <typename T>
-__device__ __forceinline__ bool chunk_feeds_residual(const ChunkParams& p) {
-  return Mma16816<T>::kSplitP && p.out_f32 != 0;
-}
-
 // The 32 rows of a warp, one per lane in registers, to rows `row` (-1 = none) of `base` by way of `stage` (128 bytes per row):
 // written as they are held, an instruction would write 16 bytes of 32 rows; from shared memory it writes contiguous bytes of a
 // few.  EB = bytes per element; columns(c, x) gives columns [c * OC, (c + 1) * OC), pack(x) makes 16 bytes of them.
@@ -357,12 +368,12 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
   long long* sm_plan = reinterpret_cast<long long*>(bars + 40);  // scan scratch, then the share's last item
   ChunkSegment* segs = reinterpret_cast<ChunkSegment*>(smem + C::kBars + 512);
-  static_assert(kSegRing == 4 && ST <= 4, "barrier layout");
+  static_assert(kSegRing == 4 && ST <= 4 && kThreadsAll / 32 <= 12, "barrier layout");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int item_tokens = NQ * p.tile_tokens;
   auto item_cost = [&](const ChunkSeq& q, int ta) {
-    const ChunkCost c = chunk_cost<D, NQ>(p, q.n - ta);
+    const ChunkCost c = chunk_cost<T, D, NQ>(p, q, ta);
     int lo, hi;
     return c.setup + c.tile * chunk_keys(p, q, ta, min(ta + item_tokens, q.n), lo, hi);
   };
@@ -375,10 +386,14 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
     const int per = (p.num_seqs + kThreadsAll - 1) / kThreadsAll;
     const int sa = min(tid * per, p.num_seqs), sb = min(sa + per, p.num_seqs);
     long long mine = 0;
+    int least = kChunkMinShare;
     for (int s = sa; s < sb; ++s) {
       const ChunkSeq q = chunk_seq(p, s, TPP);
       long long w = 0;
-      for (int ta = 0; ta < q.n; ta += item_tokens) w += item_cost(q, ta);
+      for (int ta = 0; ta < q.n; ta += item_tokens) {
+        w += item_cost(q, ta);
+        least = max(least, chunk_cost<T, D, NQ>(p, q, ta).tile);
+      }
       mine += w * vheads;
     }
     long long inc = mine;
@@ -387,7 +402,11 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       const long long up = __shfl_up_sync(0xffffffffu, inc, sh);
       if (lane >= sh) inc += up;
     }
-    if (lane == 31) sm_plan[warp] = inc;
+    least = __reduce_max_sync(0xffffffffu, least);
+    if (lane == 31) {
+      sm_plan[warp] = inc;
+      sm_plan[12 + warp] = least;
+    }
     if (tid == 0) {
       mbar_init(q_full, 1);
       mbar_init(q_empty, 1);
@@ -423,9 +442,9 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       const long long v = sm_plan[w];
       if (w < warp) before += v;
       total += v;
+      least = max(least, (int)sm_plan[12 + w]);
     }
-    long long share = (total + gridDim.x - 1) / gridDim.x;
-    if (share < kChunkMinShare) share = kChunkMinShare;
+    const long long share = max((total + gridDim.x - 1) / gridDim.x, (long long)least);
     share0 = min(share * blockIdx.x, total);
     share1 = min(share0 + share, total);
     __syncthreads();
@@ -497,10 +516,10 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       g.end = 1;
       while (more && g.end) {
         // a key tile belongs to the share that its place on the line starts in
-        const ChunkCost cost = chunk_cost<D, NQ>(p, q.n - ta);
+        const ChunkCost cost = chunk_cost<T, D, NQ>(p, q, ta);
         const long long first = at + cost.setup;
         auto tiles_before = [&](long long x) {
-          const int d = (int)min(max(x - first, 0LL), (long long)nt * cost.tile);  // (a tile count of an int32 length, times 4)
+          const int d = (int)min(max(x - first, 0LL), (long long)nt * cost.tile);  // (a tile count of an int32 length, times 14 at most)
           return (d + cost.tile - 1) / cost.tile;
         };
         const int t0 = tiles_before(share0), t1 = tiles_before(share1);
@@ -523,6 +542,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
           g.some_lo = p.window > 0 ? min(hi, max(lo, g.pos0 + g.tokens - p.window)) : lo;
           g.any_bad = 0;
           g.alternate = NQ == 2 && g.tokens <= p.tile_tokens;
+          g.residual = chunk_feeds_residual<T>(p, q, ta);
           g.slot = t0 > 0 ? 2 * (int)blockIdx.x : (t1 < nt ? 2 * (int)blockIdx.x + 1 : -1);
           if (t0 == 0 && t1 < nt && lane == 0) {
             // this CTA holds the item's first part: tell the merging kernel where the others are
@@ -636,9 +656,9 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       wait_all(&seg_full[slot], (n_seg / kSegRing) & 1);
       if (__any_sync(0xffffffffu, dead)) break;
       const ChunkSegment& sg = segs[slot];
-      const bool residual = chunk_feeds_residual<T>(p);
       const int end = uniform(sg.end), kt0 = uniform(sg.kt0), num = uniform(sg.kt1) - kt0, key_lo = uniform(sg.key_lo), key_hi = uniform(sg.key_hi);
       const int pair = NQ == 2 && !uniform(sg.alternate) ? 1 : 0;
+      const bool residual = Mma16816<T>::kSplitP && uniform(sg.residual);
       __syncwarp();
       if (lane == 0) mbar_arrive(&seg_empty[slot]);
       if (end) break;
@@ -820,7 +840,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       const int pos_a = g.pos0 + tok_first + lane_group * 32 / p.tile_heads, pos_b = g.pos0 + tok_first + (lane_group * 32 + 31) / p.tile_heads;
       const int all_hi = p.causal ? min(pos_a, g.key_cap - 1) : g.key_cap - 1;
       const int all_lo = p.window > 0 && pos_b >= p.window ? pos_b - p.window + 1 : 0;
-      const bool residual = chunk_feeds_residual<T>(p);
+      const bool residual = Mma16816<T>::kSplitP && g.residual;
       // (rows that do not exist hold other tokens' queries or whatever was there: with an infinite maximum they never ask for a
       // rescaling, whose rounding would differ from call to call)
       float m_used = row_exists ? -INFINITY : INFINITY, l_run = 0.f;

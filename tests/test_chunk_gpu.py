@@ -146,6 +146,35 @@ def test_items_of_one_and_two_row_tiles_in_turn(pal, cuda, d, tpp, hq, hkv):
             assert_chunk(_run(pal, case), case)
 
 
+SHORT_ROWS = [
+    # (new tokens, lengths, window, causal)
+    ([1] * 40, [2, 4, 8, 16] * 10, None, True),        # decode steps at the start of their sequences
+    ([1] * 24, [33, 64, 128, 255, 300, 700] * 4, None, True),
+    ([5, 9, 16, 3] * 4, [5, 20, 18, 255] * 4, None, True),
+    ([300, 70], [300, 90], None, True),                # prompts: their first rows see few keys
+    ([1, 3, 200] * 3, [900, 500, 700] * 3, 7, True),   # small windows
+    ([4, 1, 150] * 3, [4, 9, 200] * 3, None, False),
+]
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (16, 16, 64), (8, 2, 256)])
+@pytest.mark.parametrize("new,lens,window,causal", SHORT_ROWS)
+def test_short_rows_keep_to_the_parity_rule(pal, cuda, new, lens, window, causal, hq, hkv, d):
+    """The rule of the decode and prefill operators, element by element: bf16 outputs within 2e-3, or one unit in the last place, of
+    the result, for rows whose few keys average nothing out.
+
+    The residual of P leaves relative errors of at most 2^-16 of a weight, so that an output in fp32 is within 2^-16 (A + |out|) of the
+    result (A = sum p |v|, at most 6 over these draws): 2e-4, and rounded one unit in the last place away at most wherever 2e-3 is
+    less than a unit.  Rows of 256 keys and more in prompts have a standard deviation of 2^-9 / sqrt(3) * sqrt(sum p^2) * |v| =
+    1.1e-3 * 0.1 * 1 of their result: 2e-3 is 18 of them."""
+    from cases import assert_parity
+    from chunk_reference import chunk_reference
+
+    case = make_chunk_case(sum(lens) + d, new, lens, hq, hkv, d, dtype=BF16, device=cuda, window=window)
+    ref, _ = chunk_reference(case, causal)
+    assert_parity(_run(pal, case, causal=causal), ref)
+
+
 def test_scale_and_large_scores(pal, cuda):
     """Scores of hundreds: the running maximum moves, and single keys take all the weight."""
     case = make_chunk_case(15, [100, 2], [800, 1500], 8, 2, 128, dtype=BF16, device=cuda, q_scale=20.0)
