@@ -244,6 +244,12 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&s)[128]) {
   tmem_ld32(taddr + 96, d);
 }
 
+// log2 of a common factor on P and the row sum.  fp16 loses weights below 2^-25, half of its smallest step, and over 128 Ki keys a
+// 250th of the sum could go that way; weights reach 2^8 (the maximum may run that far ahead of its reference), so there is room for
+// 2^7 more below 65504, and what is lost is below 2^-32 of the largest weight.  bf16 has the exponents of fp32.
+template <typename T>
+constexpr float kChunkWeightLift = Mma16816<T>::kSplitP ? 0.f : 7.f;
+
 // P = exp2(s * scale - m_ref) of keys 64 h .. 64 h + 63 of one row, rounded to the input type, two keys to a register.  The
 // row sum is taken before the rounding.  The special-function unit (16 per clock) needs 1024 cycles for the 128 x 128
 // exponentials of a tile, as long as the tile's MMAs keep the tensor pipe.  (A part of them on the FMA pipe, as a polynomial of
@@ -959,7 +965,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
             }
           }
           if (!new_max(row_max128(sc) * p.scale_log2)) return false;
-          const float m_ref = m_used > -INFINITY ? m_used : 0.f;
+          const float m_ref = (m_used > -INFINITY ? m_used : 0.f) - kChunkWeightLift<T>;
           float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           uint32_t w[32];
           chunk_exp_half<T>(sc, 0, p.scale_log2, m_ref, w, acc);

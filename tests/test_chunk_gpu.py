@@ -175,6 +175,30 @@ def test_short_rows_keep_to_the_parity_rule(pal, cuda, new, lens, window, causal
     assert_parity(_run(pal, case, causal=causal), ref)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 200])
+def test_small_weights_of_half_precision_count(pal, cuda, d, new):
+    """One key of a tile takes the weight, with value 0; each other one has exp(-18) = 2^-26 of it and value 1.
+
+    Weights are held times 2^7 in steps of 2^-24: each off by at most 2^-32 of the largest, 127 to a tile, beside the errors of the
+    exponential (D 2^-24 * 18 * 2 + 2^-22 relative)."""
+    hkv, length, tpp = 2, 2048, 16
+    pages = length // tpp
+    k = torch.zeros((pages, hkv, d // 8, tpp, 8), dtype=FP16, device=cuda)
+    v = torch.ones((pages, hkv, d, tpp), dtype=FP16, device=cuda)
+    k[::8, :, :, 0] = 1.5   # tokens 0, 128, 256, ...
+    v[::8, :, :, 0] = 0.0
+    q = torch.full((new, 4, d), 1.5, dtype=FP16, device=cuda)
+    table = torch.arange(pages, dtype=torch.int32, device=cuda)[None]
+    lens = torch.tensor([length], dtype=torch.int32, device=cuda)
+    out = pal.paged_attention_chunk(q, k, v, table, lens, scale=8.0 / d, out_dtype=torch.float32).double()
+    seen = torch.arange(length - new, length, device=cuda) + 1
+    large = (seen + 127) // 128
+    w = torch.exp(torch.tensor(-18.0, dtype=torch.float64))
+    ref = ((seen - large) * w / (large + (seen - large) * w))[:, None, None]
+    assert ((out - ref).abs() <= 127 * 2.0 ** -32 + (36 * d * 2.0 ** -24 + 2.0 ** -22) * ref).all()
+
+
 def test_scale_and_large_scores(pal, cuda):
     """Scores of hundreds: the running maximum moves, and single keys take all the weight."""
     case = make_chunk_case(15, [100, 2], [800, 1500], 8, 2, 128, dtype=BF16, device=cuda, q_scale=20.0)
