@@ -34,6 +34,9 @@ constexpr int kThreads = 256;
 constexpr int kTokensPerTile = 64;               // list tokens a V block owns (8 where that leaves SMs idle)
 constexpr int kTileTokens = kTokensPerTile + 7;  // ... and stages: the octet that starts at its last token ends 7 later
 constexpr int kTokensPerBlock = 16;              // of a rotating block, when there are enough tokens to fill the GPU
+// Bytes of a rotating block's table of angles.  A launch has 48 KB in all without asking for more, of which the lists of a V block
+// take 1152 bytes (they are static, so every block has them).
+constexpr size_t kTableBytes = 46 * 1024;
 
 struct RotaryParams {
   RotationArgs rot;
@@ -413,13 +416,14 @@ int launch_rotary(const RotaryArgs& a, cudaStream_t stream) {
   // Sixteen tokens share a block once that gives every SM one; below, a token has blocks of its own, one per as many heads as
   // its threads hold at once while the GPU has room for them.
   const long long sms = cached_sm_count();
-  p.block_tokens = tokens >= kTokensPerBlock * sms && half <= 384 ? kTokensPerBlock : 1;  // (their table stays within 48 KB)
+  const size_t token_bytes = (size_t)2 * half * sizeof(float);
+  p.block_tokens = tokens >= kTokensPerBlock * sms && kTokensPerBlock * token_bytes <= kTableBytes ? kTokensPerBlock : 1;
   const long long groups = (tokens + p.block_tokens - 1) / p.block_tokens;
   const int units = (d + 2 * vec - 1) / (2 * vec);
   const int at_once = kThreads / units > 1 ? kThreads / units : 1;
   const long long splits_wanted = (heads + at_once - 1) / at_once, splits_room = 4 * sms / groups;
   p.head_splits = (int)(splits_room < 1 ? 1 : (splits_room < splits_wanted ? splits_room : splits_wanted));
-  size_t smem = (size_t)p.block_tokens * 2 * half * sizeof(float);
+  size_t smem = p.block_tokens * token_bytes;
   if (a.k.data) {
     p.v_tokens = tokens * a.fill.num_kv_heads >= kTokensPerTile * sms ? kTokensPerTile : 8;
     p.v_blocks = (unsigned)((tokens + p.v_tokens - 1) / p.v_tokens * a.fill.num_kv_heads);

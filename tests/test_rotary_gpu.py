@@ -54,6 +54,19 @@ def test_rotation(pal, cuda, tokens, heads, head_dim, rotary_dim, sections, orde
         assert torch.equal(out.cpu()[..., rotary_dim:], x[..., rotary_dim:])
 
 
+@pytest.mark.parametrize("pairing", ["half", "adjacent"])
+@pytest.mark.parametrize("tokens,half,head_dim", [
+    (2400, 367, 768), (2400, 368, 768), (2400, 369, 768), (2400, 375, 768), (2400, 376, 768), (2400, 384, 768),  # tables of 46 to 48 KB
+    (2400, 512, 1024), (2367, 384, 768), (5, 4096, 8192), (300, 1001, 2003),
+])
+def test_wide_heads(pal, cuda, tokens, half, head_dim, pairing):
+    """Heads up to the documented 8192 elements, whose angles fit a block's shared memory for sixteen tokens or for one."""
+    x = torch.randn((tokens, 1, head_dim), generator=torch.Generator().manual_seed(half)).to(BF16)
+    freq, pos = _freqs(half), _positions(tokens, None, 3, half)
+    out = pal.rotary_embedding(x.to(cuda), pos.to(cuda), freq.to(cuda), pairing=pairing)
+    assert_rotated(out, x, pos, freq, pairing=pairing)
+
+
 @pytest.mark.parametrize("index_dtype", [torch.int32, torch.int64, torch.int16])
 def test_far_and_negative_positions(pal, cuda, index_dtype):
     far = 30000 if index_dtype == torch.int16 else (2 ** 31 - 1 if index_dtype == torch.int32 else 2 ** 33 + 5)
