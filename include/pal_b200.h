@@ -157,9 +157,9 @@ int pal_rotary_embedding(const pal_rows* x, const pal_rows* out, const pal_rotat
 
 /* Append with rotation: the keys are rotated on their way into the K pool, the values go into the V pool as they are, and
  * (when num_q_heads > 0) the queries are rotated into queries_out, which may be queries - one launch.  Tokens are addressed
- * by slot_mapping (int64), or, when that is null, by page_table / write_positions / query_to_seq_map, with the rules of
- * pal_fill_kv_pages[_slots]: a token whose destination is out of range is skipped (its query is still rotated).
- * Destinations must differ from one another.  head_dim is a multiple of 8, at most 256. */
+ * by slot_mapping (int64), or, when that is null, by page_table (which may be null if it is empty), write_positions and
+ * query_to_seq_map, with the rules of pal_fill_kv_pages[_slots]: a token whose destination is out of range is skipped (its
+ * query is still rotated).  Destinations must differ from one another.  head_dim is a multiple of 8, at most 256. */
 int pal_fill_kv_pages_rotary(const pal_rows* new_keys, const pal_rows* new_values, const pal_rows* queries,
                              const pal_rows* queries_out, void* k_pool, void* v_pool, const int64_t* slot_mapping,
                              const void* page_table, const int32_t* write_positions, const void* query_to_seq_map,

@@ -312,7 +312,8 @@ int pal_fill_kv_pages_rotary(const pal_rows* new_keys, const pal_rows* new_value
     if (!rows_arg(what, "queries", queries, &a.q) || !rows_arg(what, "queries_out", queries_out, &o)) return PAL_ERR_BAD_ARG;
     a.q_out = RowsOut{queries_out->data, o.token_stride, o.head_stride};
   }
-  if (!slot_mapping && (!page_table || !write_positions || !query_to_seq_map) && max_pages_per_seq > 0) {
+  // (an empty page table may be null; positions and sequences are looked at before the table's width)
+  if (!slot_mapping && (!write_positions || !query_to_seq_map || (!page_table && max_pages_per_seq > 0 && num_seqs > 0))) {
     set_error("%s: slot_mapping, or page_table, write_positions and query_to_seq_map are required", what);
     return PAL_ERR_BAD_ARG;
   }

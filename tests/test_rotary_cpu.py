@@ -67,6 +67,17 @@ def test_append_arguments(lib):
         assert "fill_kv_pages_rotary" in lib.last_error()
 
 
+def test_append_addresses_are_required_whatever_the_tables_width(lib):
+    """Without slots the positions and sequences of the tokens are read even when the page table is empty: null ones are refused
+    before a launch."""
+    rows, rot = lib.Rows(4096, 32, 16), _rotation(lib)
+    for mp, seqs in ((0, 0), (0, 3), (4, 0), (4, 3)):
+        for wp, sm in ((None, None), (4096, None), (None, 4096)):
+            rc = lib.lib.pal_fill_kv_pages_rotary(rows, rows, None, None, 4096, 4096, None, 4096, wp, sm, rot, 1, seqs, 0, 1, 16, 16, 1, mp, 0, None)
+            assert rc == lib.PAL_ERR_BAD_ARG, (mp, seqs, wp, sm)
+            assert "are required" in lib.last_error()
+
+
 def test_cpu_tensors_are_rejected():
     import proxy_attention_lab_b200 as pal
 
