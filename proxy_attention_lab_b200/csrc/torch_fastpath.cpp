@@ -294,7 +294,8 @@ py::object chunk(const at::Tensor& q, const at::Tensor& k_pool, const at::Tensor
   const int64_t num_pages = v_pool.size(0), hkv = v_pool.size(1), d = v_pool.size(2), tpp = v_pool.size(3);
   const int64_t S = page_table.size(0), mp = page_table.size(1), total = q.size(0), hq = q.size(1);
   if (S == 0 || mp == 0 || total == 0 || num_pages == 0 || hkv == 0 || hq == 0 || hq % hkv != 0 || q.size(2) != d || seq_lens.numel() != S ||
-      k_pool.size(0) != num_pages || k_pool.size(1) != hkv || k_pool.size(2) * 8 != d || k_pool.size(3) != tpp || k_pool.size(4) != 8 || window < 0)
+      k_pool.size(0) != num_pages || k_pool.size(1) != hkv || k_pool.size(2) * 8 != d || k_pool.size(3) != tpp || k_pool.size(4) != 8 || window < 0 ||
+      window > 0x7fffffff)
     return py::none();
   if (cu_seqlens ? (!dense_cuda(*cu_seqlens, dev) || !int32_like(*cu_seqlens) || cu_seqlens->dim() != 1 || cu_seqlens->numel() != S + 1) : total % S != 0)
     return py::none();

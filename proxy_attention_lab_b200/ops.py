@@ -888,10 +888,12 @@ def paged_attention_chunk(queries, k_cache_pool, v_cache_pool, page_table, seque
     ``out_dtype=torch.float32``, written to ``out`` if given.  Rows that belong to no sequence (behind ``cu_seqlens[S]``) are
     not written.
     """
+    if window is not None:
+        window = min(int(window), 2 ** 31 - 1)  # (lengths are 32-bit: a wider window sees no more keys)
     if _fast is not None and stream is None and (out_dtype is None or out_dtype is torch.float32) and (window is None or (causal and window > 0)):
         try:
             done = _fast.chunk(queries, k_cache_pool, v_cache_pool, page_table, sequence_lengths, cu_seqlens, bool(causal),
-                               0 if window is None else int(window), 0.0 if scale is None else float(scale), out_dtype is torch.float32, out,
+                               window or 0, 0.0 if scale is None else float(scale), out_dtype is torch.float32, out,
                                _STATUS_PAGES)
         except TypeError:
             done = None
@@ -937,10 +939,8 @@ def paged_attention_chunk(queries, k_cache_pool, v_cache_pool, page_table, seque
     for name, t in tensors:
         if t.device != dev:
             raise ValueError(f"{name} must be on {dev}")
-    if window is not None:
-        window = int(window)
-        if window <= 0 or not causal:
-            raise ValueError("window must be positive, and needs causal attention")
+    if window is not None and (window <= 0 or not causal):
+        raise ValueError("window must be positive, and needs causal attention")
     with _Scope(dev, stream) as sp:
         if out is None:
             out = torch.empty((total, hq, d), dtype=odt, device=dev)

@@ -1,5 +1,7 @@
 """paged_attention_chunk against the definition in 64 bits."""
 
+import sys
+
 import pytest
 import torch
 
@@ -74,6 +76,17 @@ def test_float32_output(pal, cuda, d, hq, hkv):
 def test_window(pal, cuda, window, d, tpp):
     case = make_chunk_case(window, [180, 1, 5, 64], [700, 900, 130, 64], 8, 2, d, tpp=tpp, dtype=BF16, device=cuda, window=window)
     assert_chunk(_run(pal, case), case)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, sys.maxsize, 2 ** 80])
+@pytest.mark.parametrize("stream", [False, True])
+def test_windows_wider_than_any_sequence(pal, cuda, window, stream):
+    """A window past 32 bits, which is a usual way to say that there is none, through either front."""
+    case = make_chunk_case(5, [40, 1, 9, 70], [90, 700, 4, 0], 8, 2, 128, dtype=BF16, device=cuda)
+    plain = _run(pal, case).clone()
+    kw = dict(stream=torch.cuda.current_stream()) if stream else {}
+    out = pal.paged_attention_chunk(case["q"], case["k_pool"], case["v_pool"], case["table"], case["lens"], case["cu"], window=window, **kw)
+    assert torch.equal(out.view(torch.int16), plain.view(torch.int16))
 
 
 @pytest.mark.parametrize("d", [128, 256, 32])
