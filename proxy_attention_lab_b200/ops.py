@@ -425,9 +425,9 @@ def fill_kv_pages_rotary(
     if (_fast is not None and stream is None and inplace and queries_out is None and pairing in ROTARY_PAIRING and section_order in SECTION_ORDER
             and (slot_mapping is None or page_table is None)):
         try:
-            done = _fast.fill_rotary(new_keys, new_values, global_key_pool, global_value_pool, page_table if slot_mapping is None else slot_mapping,
-                                     current_token_write_positions, query_to_seq_map, positions, inv_freq, sections, SECTION_ORDER[section_order],
-                                     ROTARY_PAIRING[pairing], magnitude, queries)
+            where = (page_table, current_token_write_positions, query_to_seq_map) if slot_mapping is None else (slot_mapping, None, None)
+            done = _fast.fill_rotary(new_keys, new_values, global_key_pool, global_value_pool, *where, positions, inv_freq, sections,
+                                     SECTION_ORDER[section_order], ROTARY_PAIRING[pairing], magnitude, queries)
         except TypeError:
             done = None
         if done is not None:

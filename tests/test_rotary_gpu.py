@@ -303,6 +303,27 @@ def test_tokens_without_a_destination_are_skipped(pal, cuda):
     assert torch.equal(dv.cpu(), expect)
 
 
+@pytest.mark.parametrize("named_stream", [False, True])
+@pytest.mark.parametrize("index_dtype", [torch.int32, torch.int64])
+def test_slots_come_before_other_addresses(pal, cuda, index_dtype, named_stream):
+    """Slots [sequences, tokens] beside write positions, a sequence map and a page table that say something else: the slots count."""
+    B, L, hkv, D, tpp, pages = 4, 6, 2, 64, 16, 32
+    g = torch.Generator().manual_seed(8)
+    k, v = (torch.randn((B * L, hkv, D), generator=g).to(BF16).to(cuda) for _ in range(2))
+    slots = torch.randperm(pages * tpp, generator=g)[:B * L].reshape(B, L)
+    pos = torch.arange(L, dtype=torch.int32).repeat(B).to(cuda)
+    seq = torch.arange(B, dtype=torch.int32).repeat_interleave(L).to(cuda)
+    freq = _freqs(32).to(cuda)
+    pools = lambda: (torch.zeros((pages, hkv, D // 8, tpp, 8), dtype=BF16, device=cuda), torch.zeros((pages, hkv, D, tpp), dtype=BF16, device=cuda))
+    expect = pal.fill_kv_pages_rotary(k, v, *pools(), slots.flatten().to(torch.int64).to(cuda), inv_freq=freq, positions=pos)
+    kw = dict(stream=torch.cuda.current_stream()) if named_stream else {}
+    table = torch.arange(B, dtype=torch.int32, device=cuda)[:, None]
+    for page_table in (None, table):
+        got = pal.fill_kv_pages_rotary(k, v, *pools(), page_table, pos, seq, slot_mapping=slots.to(index_dtype).to(cuda), inv_freq=freq, positions=pos, **kw)
+        for a, b in zip(got, expect):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
 def test_queries_in_place_of_a_fused_projection(pal, cuda):
     T, hq, hkv, D, tpp = 90, 4, 2, 128, 16
     table, pages, seq, pos = _batch([T], [2], tpp)
