@@ -357,8 +357,9 @@ int pal_paged_attention_prefill_ragged(const void* q_prompt, const void* k_promp
  * It sees the keys up to its own position, and with window > 0 only the last `window` of them; with causal = 0 (window must
  * be 0) all L keys.  A row that sees no key becomes zeros.  out [total_tokens, Hq, D] in the query dtype, or float32 with
  * dtype | PAL_OUT_F32; rows that belong to no sequence are left as they were.  Page ids are clamped to [0, num_pages); pages
- * that hold no visible key are not read.  scale <= 0 selects 1/sqrt(D).  Keys and values that are not finite reach the rows
- * that see them alone (an infinite value makes such a row NaN), slots that no row sees may hold anything.
+ * that hold no visible key are not read.  scale <= 0 selects 1/sqrt(D).  An element of a value that is not finite makes that
+ * element of the rows that see it an infinity or NaN, and no other; a key that is not finite reaches the rows that see it
+ * alone; slots that no row sees may hold anything.
  *
  * scratch: pal_chunk_scratch_bytes() bytes of device memory, 256-byte aligned, with any contents, for one call at a time.
  * status: one 32-bit word of device memory that is zero before the first use and takes the error code of a wait that gave

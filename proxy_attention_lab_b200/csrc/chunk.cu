@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const Chu
 #pragma unroll
         for (int u = 0; u < kMergeParts; ++u) {
           const float wu = __shfl_sync(0xffffffffu, w, (j + u) & 31);
-          if (j + u < count && wu != 0.f)
+          if (j + u < count)  // (a part without keys holds zeros; one of no weight may hold an infinity)
 #pragma unroll
             for (int i = 0; i < NV; ++i)
               if (i * 128 + lane * 4 < head_dim) {

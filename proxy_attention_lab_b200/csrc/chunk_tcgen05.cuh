@@ -78,6 +78,7 @@ struct ChunkSegment : ChunkWork {
 
 struct ChunkParams {
   const void* k_pool;
+  const void* v_pool;
   const uint32_t* page_table;
   const int32_t* seq_lens;
   const int32_t* cu_seqlens;  // null = every sequence has tokens_per_seq rows
@@ -338,6 +339,39 @@ __device__ __forceinline__ void chunk_store_rows(unsigned char* stage, int lane,
       if (to[it] >= 0) *reinterpret_cast<uint4*>(base + (size_t)to[it] * (D * EB) + (c * kPieces + piece) * 16) = v[it];
     }
     __syncwarp();
+  }
+}
+
+// Adds the values that are not finite and were zeroed for other rows' sake to the stored row of token `tok` of the item and head `head`
+// of the tile, where it sees their keys.  A rare path, so a function of its own in rolled loops: inlined, its registers cost the hot
+// loop 60 bytes of spills and chunks of a prompt 1.4 %.
+template <typename T, int D, int TPP>
+__device__ __noinline__ void chunk_add_bad_values(const ChunkParams& p, const ChunkSegment& g, int tok, int head) {
+  const int pos = g.pos0 + tok;
+  const int hi = p.causal ? min(pos, g.key_cap - 1) : g.key_cap - 1, lo = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
+  const bool direct = g.slot < 0, f32 = !direct || p.out_f32;
+  const size_t at = (direct ? (size_t)(g.row0 + tok) * p.num_q_heads + g.head0 + head : (size_t)g.slot * p.part_rows + tok * p.tile_heads + head) * D;
+  float* out32 = (direct ? static_cast<float*>(p.out) : p.part_acc) + at;
+  T* out16 = static_cast<T*>(p.out) + at;
+#pragma unroll 1
+  for (int k = 0; k < 24; ++k) {
+    const int key0 = ((k < 12 ? g.some_hi / kTile : g.key_lo / kTile - 3) + (k >> 2)) * kTile + (k & 3) * 32;
+#pragma unroll 1
+    for (uint32_t left = g.bad[k >> 2][k & 3]; left; left &= left - 1) {
+      const int key = key0 + __ffs(left) - 1;
+      if (key < lo || key > hi) continue;
+      const long long page = min((long long)p.page_table[(size_t)g.seq * p.max_pages_per_seq + key / TPP], p.num_pages - 1);
+      const T* v = static_cast<const T*>(p.v_pool) + ((size_t)page * p.num_kv_heads + g.kv_head) * (D * TPP) + key % TPP;
+#pragma unroll 1
+      for (int d = 0; d < D; ++d) {
+        const float x = Mma16816<T>::to_float(v[d * TPP]);
+        if (isfinite(x)) continue;
+        if (f32)
+          out32[d] += x;
+        else
+          out16[d] = Mma16816<T>::from_float(Mma16816<T>::to_float(out16[d]) + x);
+      }
+    }
   }
 }
 
@@ -882,7 +916,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
         // Values that a row does not see are multiplied by P = 0, which is not 0 if they hold an infinity or a NaN.  So, in the
         // 16-key steps that are used: slots that no row of the item sees (past the last key, before the window, never written)
         // are zeroed; a value that some rows see and others do not is zeroed if it is not finite, and its key noted: the rows
-        // that see it come out as NaN.  (Values that all rows see need no care.)
+        // that see it have it added to their output.  (Values that all rows see need no care.)
         auto clear_values = [&]() {
           const int c_lo = max(0, g.key_lo - j * kTile), c_hi = min(kTile, g.key_hi - j * kTile);
           const int some_lo = g.some_lo - j * kTile, some_hi = g.some_hi - j * kTile;
@@ -1016,20 +1050,8 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
       const bool nan = mine > 0 && l_run != l_run;
       const bool any = mine > 0 && (m_used > -INFINITY || nan);
       float m_row = any ? (nan ? fmaxf(m_used, 0.f) : m_used) : -INFINITY, l_row = any ? l_run : 0.f;
-      auto poisoned = [&]() {  // this row sees a key whose value is not finite
-        bool bad = false;
-#pragma unroll 1
-        for (int k = 0; k < 24; ++k) {
-          const uint32_t word = g.bad[k >> 2][k & 3];
-          const int key0 = ((k < 12 ? g.some_hi / kTile : g.key_lo / kTile - 3) + (k >> 2)) * kTile + (k & 3) * 32;
-          for (uint32_t left = word; left; left &= left - 1) {
-            const int key = key0 + __ffs(left) - 1;
-            bad = bad || (key >= lo && key <= hi);
-          }
-        }
-        return bad;
-      };
       float w_own = any ? 1.f : 0.f, w_other = 0.f;
+      bool any_other = false;  // ... and in the second accumulator, once it has been merged
       const int used_rows = tile_tokens * p.tile_heads;
       const bool merge = alt && num > 1;  // with a single key tile the second accumulator has nothing
       // the buffer holds kMergeRows rows: one pass, or two when it is 64 and more rows are in use
@@ -1070,11 +1092,11 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
               const float2 ml = sMl[row % C::kMergeRows];
               const float m = fmaxf(m_row, ml.x);
               w_own = m_row > -INFINITY ? fast_exp2(m_row - m) : 0.f;
-              w_other = ml.x > -INFINITY ? fast_exp2(ml.x - m) : 0.f;
+              any_other = ml.x > -INFINITY;
+              w_other = any_other ? fast_exp2(ml.x - m) : 0.f;
               l_row = l_row * w_own + ml.y * w_other;
               m_row = m;
             }
-            if (g.any_bad && poisoned()) l_row = __int_as_float(0x7fffffff);
             const bool direct = g.slot < 0;
             const float inv = direct ? chunk_inverse_sum(l_row) : 1.f;
             const float f0 = w_own * inv, f1 = w_other * inv;
@@ -1088,8 +1110,8 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
               tmem_wait_ld();
               // (a row whose O counts for nothing may hold anything: no key seen, or no PV run at all)
 #pragma unroll
-              for (int k = 0; k < OC; ++k) x[k] = f0 != 0.f ? __uint_as_float(v[k / kOC][k % kOC]) * f0 : 0.f;
-              if (merge && f1 != 0.f) {
+              for (int k = 0; k < OC; ++k) x[k] = any ? __uint_as_float(v[k / kOC][k % kOC]) * f0 : 0.f;
+              if (any_other) {
 #pragma unroll
                 for (int k = 0; k < OC / 4; ++k) {
                   const float4 y = *merge_chunk(c * (OC / 4) + k);
@@ -1112,6 +1134,8 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
                                                                return make_uint4(Mma16816<T>::pack(x[0], x[1]), Mma16816<T>::pack(x[2], x[3]),
                                                                                  Mma16816<T>::pack(x[4], x[5]), Mma16816<T>::pack(x[6], x[7]));
                                                              });
+            if (g.any_bad && row_exists)  // (the stores above end with a warp-wide barrier)
+              chunk_add_bad_values<T, D, TPP>(p, g, tok_first + tok, head);
           }
           if (merge) {
             __syncwarp();
@@ -1155,6 +1179,7 @@ template <int D, int TPP>
 int launch_chunk_shape(const ChunkArgs& a, cudaStream_t stream) {
   ChunkParams p;
   p.k_pool = a.k_pool;
+  p.v_pool = a.v_pool;
   p.page_table = a.page_table;
   p.seq_lens = a.seq_lens;
   p.cu_seqlens = a.cu_seqlens;

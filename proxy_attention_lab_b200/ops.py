@@ -881,8 +881,8 @@ def paged_attention_chunk(queries, k_cache_pool, v_cache_pool, page_table, seque
     ``i`` of ``n`` stands at position ``L - n + i`` and sees the keys up to its own position, only the last ``window`` of them
     when a window is given, or all ``L`` keys with ``causal=False``.  A row that sees no key becomes zeros.  Counts from a
     single token (a decode step) to a whole prompt may be mixed; no length is read back to the host.
-    Values that are not finite reach the rows that see them alone (an infinite one makes such a row NaN); slots that no row sees
-    may hold anything.
+    An element of a value that is not finite makes that element of the rows that see it an infinity or NaN, and no other; a key
+    that is not finite reaches the rows that see it alone; slots that no row sees may hold anything.
 
     ``queries`` may be a strided view.  Returns ``[T, Hq, D]`` in the query dtype, or in float32 with
     ``out_dtype=torch.float32``, written to ``out`` if given.  Rows that belong to no sequence (behind ``cu_seqlens[S]``) are

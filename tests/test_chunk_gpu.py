@@ -437,6 +437,49 @@ def test_values_a_row_does_not_see_do_not_reach_it(pal, cuda, dtype, value, hq, 
         assert 0 < int((~torch.isfinite(out.float()).all(-1)).any(-1).sum()) < sum(new)
 
 
+@pytest.mark.parametrize("dtype,out_dtype", [(BF16, None), (FP16, None), (BF16, torch.float32), (FP16, torch.float32)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("hq,hkv,d,tpp", [(8, 2, 128, 16), (2, 2, 64, 32), (4, 1, 256, 16), (3, 1, 80, 32)])
+def test_values_that_are_not_finite_stay_in_their_elements(pal, cuda, dtype, out_dtype, value, hq, hkv, d, tpp):
+    """An element of a value that is not finite makes that element of the rows that see it not finite and leaves all others bit for
+    bit as they were, wherever the key lies: seen by all rows of an item, by some, in a part that is merged."""
+    new, lens = [300, 5, 40, 1, 2], [430, 900, 40, 20000, 7]
+    kw = dict(out_dtype=out_dtype)
+    for window in (None, 150):
+        case = make_chunk_case(35, new, lens, hq, hkv, d, tpp=tpp, dtype=dtype, device=cuda, window=window)
+        clean = _run(pal, case, **kw).clone()
+        # (sequence, token, kv head, element)
+        spots = [(0, 200, 0, 3), (0, 429, hkv - 1, d - 1), (0, 131, 0, 17), (0, 257, hkv - 1, 17), (1, 898, 0, 8), (2, 17, 0, 0), (4, 6, 0, 31)]
+        spots += [(0, 30, 0, 5), (0, 60, hkv - 1, 9)] if window else [(0, 2, 0, 5), (1, 100, 0, 20), (3, 12345, hkv - 1, 21), (3, 7, 0, 22)]
+        hit = torch.zeros(clean.shape, dtype=torch.bool, device=cuda)
+        for s, token, head, element in spots:
+            page = int(case["table"][s, token // tpp])
+            case["v_pool"][page, head, element, token % tpp] = value
+            pos = torch.arange(lens[s] - new[s], lens[s], device=cuda)
+            sees = (pos >= token) & ((pos - token < window) if window else True)
+            rows = hit[sum(new[:s]):sum(new[:s + 1]), head * (hq // hkv):(head + 1) * (hq // hkv), element]
+            rows |= sees[:, None]
+        assert hit.any()
+        for _ in range(2):
+            out = _run(pal, case, **kw)
+            assert not torch.isfinite(out[hit]).any()
+            assert torch.equal(out[~hit], clean[~hit])
+            if value != value:
+                assert torch.isnan(out[hit]).all()
+
+
+def test_infinities_of_both_signs_meet(pal, cuda):
+    """In fp16 (no second product whose weights may be zero) an infinity that some rows of the item see stays one, and two of
+    opposite signs make a NaN."""
+    case = make_chunk_case(36, [100], [100], 4, 1, 64, dtype=FP16, device=cuda)
+    for token, element, value in ((10, 3, float("inf")), (70, 3, -float("inf")), (40, 5, -float("inf"))):
+        case["v_pool"][int(case["table"][0, token // 16]), 0, element, token % 16] = value
+    out = _run(pal, case).float()
+    assert torch.isfinite(out[:10]).all()
+    assert (out[10:70, :, 3] == float("inf")).all() and torch.isnan(out[70:, :, 3]).all() and (out[40:, :, 5] == -float("inf")).all()
+    assert torch.isfinite(out[..., 6:]).all()
+
+
 @pytest.mark.parametrize("d,tpp", [(64, 16), (128, 32), (256, 16)])
 @pytest.mark.parametrize("length", [1, 33, 129, 300])
 def test_keys_that_are_not_numbers(pal, cuda, d, tpp, length):
