@@ -17,6 +17,7 @@
 // prefill append looks like - their K vectors are contiguous per (head, chunk) and their V elements are
 // 4, 8 or 16 contiguous bytes per (head, d): the tokens are staged in shared memory and written back
 // transposed with one wide store per chunk.  Groups without any such chunk take the scattered path.
+#include "append.cuh"
 #include "common.cuh"
 #include "launch.h"
 
@@ -75,37 +76,6 @@ __global__ void __launch_bounds__(256) fill_kv_pages_kernel(
 
 
 constexpr int kGroupTokens = 16;
-
-__device__ __forceinline__ void cp_async_16(void* smem_dst, const void* gmem_src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem_dst)), "l"(gmem_src)
-               : "memory");
-}
-
-// (page, slot) of token t, or page = -1 when the token has to be skipped
-template <bool kSlots>
-__device__ __forceinline__ void token_destination(long long t, const int64_t* slot_mapping, const uint32_t* page_table,
-                                                  const int32_t* write_positions, const uint32_t* query_to_seq_map,
-                                                  int num_seqs, int tokens_per_page, long long num_pages,
-                                                  int max_pages_per_seq, long long& page, int& slot) {
-  page = -1;
-  slot = 0;
-  if (kSlots) {
-    const long long s = slot_mapping[t];
-    if (s < 0 || s >= num_pages * tokens_per_page) return;
-    page = s / tokens_per_page;
-    slot = (int)(s - page * tokens_per_page);
-  } else {
-    const uint32_t seq = query_to_seq_map[t];
-    const int pos = write_positions[t];
-    if (pos < 0 || seq >= (uint32_t)num_seqs) return;
-    const int block = pos / tokens_per_page;
-    if (block >= max_pages_per_seq) return;
-    const long long pg = page_table[(long long)seq * max_pages_per_seq + block];
-    if (pg >= num_pages) return;
-    page = pg;
-    slot = pos - block * tokens_per_page;
-  }
-}
 
 template <bool kSlots>
 __global__ void __launch_bounds__(256) fill_kv_pages_grouped_kernel(

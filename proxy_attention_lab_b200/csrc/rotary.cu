@@ -24,6 +24,7 @@
 //     ldmatrix.trans does the transposition: its row addresses are free, so row 2 t + b of matrix k is given the address of
 //     token 2 k + b of octet t, and each lane receives the eight tokens of one head-dim element of octet t in four
 //     registers - one 16-byte store.  The rest (single tokens, ends of runs) leaves in 2-byte stores.
+#include "append.cuh"
 #include "common.cuh"
 #include "launch.h"
 
@@ -143,26 +144,13 @@ __device__ __forceinline__ void turn(Elems<T, V>& a, Elems<T, V>& b, const Angle
   }
 }
 
-// (page, slot) of token t, or page = -1 when the token is skipped: the rules of fill_kv_pages
+// (page, slot) of token t, or page = -1 when the token has to be skipped
 __device__ __forceinline__ void destination(const FillArgs& f, long long t, long long& page, int& slot) {
-  page = -1;
-  slot = 0;
-  if (f.slot_mapping) {
-    const long long s = f.slot_mapping[t];
-    if (s < 0 || s >= f.num_pages * f.tokens_per_page) return;
-    page = s / f.tokens_per_page;
-    slot = (int)(s - page * f.tokens_per_page);
-  } else {
-    const uint32_t seq = static_cast<const uint32_t*>(f.query_to_seq_map)[t];
-    const int pos = f.write_positions[t];
-    if (pos < 0 || seq >= (uint32_t)f.num_seqs) return;
-    const int block = pos / f.tokens_per_page;
-    if (block >= f.max_pages_per_seq) return;
-    const long long pg = static_cast<const uint32_t*>(f.page_table)[(long long)seq * f.max_pages_per_seq + block];
-    if (pg >= f.num_pages) return;
-    page = pg;
-    slot = pos - block * f.tokens_per_page;
-  }
+  const uint32_t *table = static_cast<const uint32_t*>(f.page_table), *map = static_cast<const uint32_t*>(f.query_to_seq_map);
+  if (f.slot_mapping)
+    token_destination<true>(t, f.slot_mapping, table, f.write_positions, map, f.num_seqs, f.tokens_per_page, f.num_pages, f.max_pages_per_seq, page, slot);
+  else
+    token_destination<false>(t, f.slot_mapping, table, f.write_positions, map, f.num_seqs, f.tokens_per_page, f.num_pages, f.max_pages_per_seq, page, slot);
 }
 
 // A rotating block: tokens [t0, t0 + block_tokens) of heads [head0, head1), counting the queries' heads first and then the
@@ -254,16 +242,6 @@ __device__ __forceinline__ void rotate(const RotaryParams& p, unsigned block, fl
   }
 }
 
-__device__ __forceinline__ void copy_async_16(uint32_t smem_dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void ldmatrix_x4_transposed(uint32_t (&r)[4], uint32_t saddr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(saddr)
-               : "memory");
-}
-
 // One V block: tokens [t0, t0 + 64) of one head.  A staged row is padded to whole groups of eight 16-byte chunks, and chunk c
 // of row r sits at c ^ swizzle(r): the eight rows one ldmatrix phase reads are tokens b + 8 t (b < 2, t < 4), which the
 // swizzle sends to eight different banks.
@@ -290,7 +268,7 @@ __device__ __forceinline__ void move_values(const RotaryParams& p, unsigned bloc
   if (p.v_vec) {
     for (int i = tid; i < rows * chunks; i += kThreads) {
       const int r = i / chunks, c = i - r * chunks;
-      copy_async_16(sbase + r * pitch + ((c ^ row_swizzle(r)) << 4), src + r * p.src_v.token_stride + c * 8);
+      cp_async_16(smem + r * pitch + ((c ^ row_swizzle(r)) << 4), src + r * p.src_v.token_stride + c * 8);
     }
   } else {
     for (int i = tid; i < rows * f.head_dim; i += kThreads) {
@@ -336,7 +314,7 @@ __device__ __forceinline__ void move_values(const RotaryParams& p, unsigned bloc
     const int k = lane >> 3, row_t = (lane & 7) >> 1, row_b = lane & 1;
     const int row = s_octet[min(4 * q4 + row_t, num_octets - 1)] + 2 * k + row_b;
     uint32_t v[4];
-    ldmatrix_x4_transposed(v, sbase + row * pitch + ((c ^ row_swizzle(row)) << 4));
+    ldmatrix_x4_trans(v, sbase + row * pitch + ((c ^ row_swizzle(row)) << 4));
     const int mine = 4 * q4 + (lane & 3), d = 8 * c + (lane >> 2);
     if (mine < num_octets) {
       const int first = s_octet[mine] + 1;
