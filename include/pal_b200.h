@@ -121,8 +121,9 @@ int pal_fill_kv_pages_slots(const void* new_keys, const void* new_values, void* 
  *
  * Frequency i < num_freqs turns one pair of elements (a, b) of every head of token t by the angle
  * positions[axis(i)][t] * inv_freq[i]: a' = magnitude * (a cos - b sin), b' = magnitude * (b cos + a sin).
- * Elements from 2 * num_freqs on pass through unchanged.  The angle is formed and reduced in 64 bits, so that far
- * positions keep the accuracy of near ones; the rotation is fp32, rounded once. */
+ * Elements from 2 * num_freqs on pass through unchanged.  The angle is formed and reduced in 64 bits, so that
+ * positions up to 2^29 keep the accuracy of near ones (6e-7 rad are lost at 2^31, and in proportion beyond); the rotation is
+ * fp32, rounded once. */
 #define PAL_PAIRING_HALF 0        /* the pair of frequency i is elements (i, i + num_freqs) */
 #define PAL_PAIRING_ADJACENT 1    /* ... elements (2i, 2i + 1) */
 #define PAL_SECTIONS_BLOCKED 0    /* axis 0 has the first sections[0] frequencies, axis 1 the next sections[1], ... */

@@ -6,7 +6,8 @@
 // with (a, b) = elements (i, i + R/2) or (2i, 2i + 1), and m a common magnitude.  Elements past R pass through.
 // The angle of a far position is large (position 10^6 times frequency 1), and its fp32 product would be off by up to
 // 2^-24 * 10^6 = 0.06 rad, so product and reduction to a fraction of a turn are taken in fp64 (exact product for
-// positions below 2^29); the fraction, at most half a turn, is then good to 2^-25 turns in fp32 and sincospif does the rest.
+// positions below 2^29; above, product and factor are off by 3e-16 of the angle, 1e-7 turns at 2^31); the fraction, at most half a
+// turn, is then good to 2^-25 turns in fp32 and sincospif does the rest.
 //
 // Bound: memory.  A rotated element costs 4 bytes of traffic and ~3 flops; the angle, ~60 instructions, is shared by all
 // heads of a token.  So a block takes a few tokens, computes their sines and cosines once into shared memory, and then a

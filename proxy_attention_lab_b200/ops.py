@@ -147,7 +147,7 @@ def resolve_partition_pages(partition_pages, S, hq, hkv, d, tpp, max_pages) -> i
 
 def check_status(stream=None, device=None) -> None:
     """Raise ``RuntimeError`` if a kernel of the last call on this (device, stream) gave up a bounded wait, or one of any chunk
-    call on this device did.
+    call on this device did (but for replays of a chunk call that was captured before the first one outside a capture).
 
     Synchronises with the stream; meant for tests and debugging."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
@@ -358,7 +358,7 @@ def rotary_embedding(x, positions, inv_freq, *, sections=None, section_order: st
     sign), or ``[A, T]`` with ``sections``, the number of frequencies that each of the ``A <= 4`` axes (time, height, width,
     ...) turns: the first ``sections[0]`` belong to axis 0 and so on (``section_order="blocked"``), or frequency ``i``
     belongs to axis ``i % A`` until that axis has its number, and the rest to axis 0 (``"interleaved"``).  The angle is
-    taken in 64 bits, so far positions are as accurate as near ones.
+    taken in 64 bits, so positions up to 2^29 are as accurate as near ones (6e-7 rad are lost at 2^31, and in proportion beyond).
 
     ``x`` may be a strided view (a column range of a fused projection); the result is contiguous, or ``out`` (which may be
     ``x``, but must not overlap it otherwise).  Negated positions undo the rotation; the gradient of ``x`` is the rotation of
