@@ -343,8 +343,8 @@ __device__ __forceinline__ void chunk_store_rows(unsigned char* stage, int lane,
 }
 
 // Adds the values that are not finite and were zeroed for other rows' sake to the stored row of token `tok` of the item and head `head`
-// of the tile, where it sees their keys.  A rare path, so a function of its own in rolled loops: inlined, its registers cost the hot
-// loop 60 bytes of spills and chunks of a prompt 1.4 %.
+// of the tile, where it sees their keys.  A rare path, so a function of its own: inlined, its registers cost the hot loop 60 bytes of
+// spills and chunks of a prompt 1.4 %.
 template <typename T, int D, int TPP>
 __device__ __noinline__ void chunk_add_bad_values(const ChunkParams& p, const ChunkSegment& g, int tok, int head) {
   const int pos = g.pos0 + tok;
@@ -354,24 +354,44 @@ __device__ __noinline__ void chunk_add_bad_values(const ChunkParams& p, const Ch
   float* out32 = (direct ? static_cast<float*>(p.out) : p.part_acc) + at;
   T* out16 = static_cast<T*>(p.out) + at;
 #pragma unroll 1
-  for (int k = 0; k < 24; ++k) {
-    const int key0 = ((k < 12 ? g.some_hi / kTile : g.key_lo / kTile - 3) + (k >> 2)) * kTile + (k & 3) * 32;
+  for (int k = 0; k < 96; ++k) {  // groups of eight keys, which the V pool keeps side by side
+    uint32_t left = (g.bad[k >> 4][(k >> 2) & 3] >> ((k & 3) * 8)) & 0xffu;
+    if (left == 0) continue;
+    const int key0 = ((k < 48 ? g.some_hi / kTile : g.key_lo / kTile - 3) + (k >> 4)) * kTile + (k & 15) * 8;
+    if (key0 < lo) left &= 0xffu << min(lo - key0, 8);
+    if (key0 + 7 > hi) left &= 0xffu >> min(key0 + 7 - hi, 8);
+    if (left == 0) continue;
+    const long long page = min((long long)p.page_table[(size_t)g.seq * p.max_pages_per_seq + key0 / TPP], p.num_pages - 1);
+    const T* v = static_cast<const T*>(p.v_pool) + ((size_t)page * p.num_kv_heads + g.kv_head) * (D * TPP) + key0 % TPP;
+    int nans = 0;
 #pragma unroll 1
-    for (uint32_t left = g.bad[k >> 2][k & 3]; left; left &= left - 1) {
-      const int key = key0 + __ffs(left) - 1;
-      if (key < lo || key > hi) continue;
-      const long long page = min((long long)p.page_table[(size_t)g.seq * p.max_pages_per_seq + key / TPP], p.num_pages - 1);
-      const T* v = static_cast<const T*>(p.v_pool) + ((size_t)page * p.num_kv_heads + g.kv_head) * (D * TPP) + key % TPP;
-#pragma unroll 1
-      for (int d = 0; d < D; ++d) {
-        const float x = Mma16816<T>::to_float(v[d * TPP]);
-        if (isfinite(x)) continue;
+    for (int d0 = 0; d0 < D; d0 += 4) {
+      uint4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const uint4*>(v + (d0 + i) * TPP);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        float sum = 0.f;
+        bool found = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float2 pair = Mma16816<T>::unpack(w[e >> 1]);
+          const float f = e & 1 ? pair.y : pair.x;
+          if ((left >> e & 1) && !isfinite(f)) {
+            sum += f;
+            found = true;
+          }
+        }
+        if (!found) continue;
+        nans += isnan(sum);
         if (f32)
-          out32[d] += x;
+          out32[d0 + i] += sum;
         else
-          out16[d] = Mma16816<T>::from_float(Mma16816<T>::to_float(out16[d]) + x);
+          out16[d0 + i] = Mma16816<T>::from_float(Mma16816<T>::to_float(out16[d0 + i]) + sum);
       }
     }
+    if (nans == D) return;  // (whole tokens that are not numbers: nothing changes the row any more)
   }
 }
 
@@ -1134,7 +1154,7 @@ __global__ void __launch_bounds__(128 + 128 * NQ, 1)
                                                                return make_uint4(Mma16816<T>::pack(x[0], x[1]), Mma16816<T>::pack(x[2], x[3]),
                                                                                  Mma16816<T>::pack(x[4], x[5]), Mma16816<T>::pack(x[6], x[7]));
                                                              });
-            if (g.any_bad && row_exists)  // (the stores above end with a warp-wide barrier)
+            if (g.any_bad && row_exists && l_row == l_row)  // (the stores above end with a warp-wide barrier; a row of NaN stays one)
               chunk_add_bad_values<T, D, TPP>(p, g, tok_first + tok, head);
           }
           if (merge) {
