@@ -884,6 +884,9 @@ def paged_attention_chunk(queries, k_cache_pool, v_cache_pool, page_table, seque
     An element of a value that is not finite makes that element of the rows that see it an infinity or NaN, and no other; a key
     that is not finite reaches the rows that see it alone; slots that no row sees may hold anything.
 
+    The weights of a row are rounded to the query dtype for the product with the values; in bfloat16 the remainder is added for
+    rows of fewer than 256 keys and for float32 outputs.
+
     ``queries`` may be a strided view.  Returns ``[T, Hq, D]`` in the query dtype, or in float32 with
     ``out_dtype=torch.float32``, written to ``out`` if given.  Rows that belong to no sequence (behind ``cu_seqlens[S]``) are
     not written.
